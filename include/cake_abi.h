@@ -37,6 +37,7 @@ extern "C" {
 
 #define CAKE_DTYPE_F32 0
 #define CAKE_DTYPE_BF16 1
+#define CAKE_DTYPE_F16 2 /* row quantisation inputs only */
 
 /* ---------------------------------------------------------------- general */
 
@@ -285,6 +286,64 @@ int32_t cake_rpa_decode_static_scratch(const cake_rpa_desc* desc, const void* q,
 
 int32_t cake_rpa_status(cake_rpa* plan, void* stream, cake_status* out);
 int32_t cake_rpa_launches_per_enqueue(const cake_rpa* plan);
+
+/* ---------------------------------------------------------------- the 8-bit linear layer
+ * No counterpart in the reference, whose matmul is bf16 only. Operands are e4m3 codes [rows, cols]
+ * (cols contiguous) with one scale per 128 consecutive columns of a row (the last group of a row may be
+ * shorter): scales are e8m0 bytes [rows, ceil(cols / 128)], byte b standing for 2^(b - 127), 255 for NaN.
+ *
+ * A group's scale is the least power of two s >= 2^-127 with max |v| <= 448 s; 1 where the group is
+ * all zeros; NaN, with NaN codes throughout, where the group holds an infinity or a NaN. A code is v / s
+ * rounded to nearest even. Row strides count elements (bytes for codes and scales); a stride is not looked
+ * at when there is one row. rows may be 0: nothing is launched and no pointer looked at. Any alignment of
+ * x to its elements is taken; 16-byte aligned rows are faster. */
+
+#define CAKE_GATE_NONE 0
+#define CAKE_GATE_SILU 1 /* x is [rows, 2 cols]: gate | up; v = gate / (1 + exp(-gate)) * up */
+
+/* x: dtype [rows, cols] -> q, scales. Nothing but the groups' own codes and scales is written. */
+int32_t cake_quantize_rows_enqueue(const void* x, int32_t dtype, int64_t x_row_stride, int32_t gate,
+                                   int64_t rows, int64_t cols, void* q, int64_t q_row_stride,
+                                   void* scales, int64_t scales_row_stride, void* stream);
+
+/* h = x + residual (residual NULL: h = x), in 32 bits; residual_out = h rounded to dtype (NULL without a
+ * residual; may be residual or x itself); v = h / sqrt(mean(h^2) + epsilon) * weight -> q, scales.
+ * weight: [cols], of the type of x or f32. */
+#define CAKE_RMS_NORM_MAX_COLUMNS 32768
+int32_t cake_rms_norm_quantize_enqueue(const void* x, int32_t dtype, int64_t x_row_stride,
+                                       const void* residual, int64_t residual_row_stride,
+                                       void* residual_out, int64_t residual_out_row_stride,
+                                       const void* weight, int32_t weight_dtype, float epsilon,
+                                       int64_t rows, int64_t cols, void* q, int64_t q_row_stride,
+                                       void* scales, int64_t scales_row_stride, void* stream);
+
+/* out[m, n] = sum over k of lhs[m, k] * s_lhs[m, k / 128] * rhs[n, k] * s_rhs[n, k / 128], accumulated in
+ * f32 and rounded once to out_dtype. One plan serves any number of rows m. */
+typedef struct cake_scaled_matmul_desc {
+  int64_t n;         /* rows of rhs = columns of out */
+  int64_t k;         /* contraction */
+  int32_t out_dtype; /* CAKE_DTYPE_F32 or CAKE_DTYPE_BF16 */
+  int32_t tile;      /* 0 = library default; 128, 192, 224: columns of a 128-row output tile;
+                        16, 32, 64: tokens of a tile of 128 rhs rows (few rows m) */
+  int32_t k_split;   /* 0 = library default; with tile 16, 32 or 64: 1..8 blocks share a tile's contraction */
+  int32_t reserved;  /* 0 */
+} cake_scaled_matmul_desc;
+
+typedef struct cake_scaled_matmul cake_scaled_matmul;
+
+int32_t cake_scaled_matmul_create(const cake_scaled_matmul_desc* desc, cake_scaled_matmul** out);
+int32_t cake_scaled_matmul_destroy(cake_scaled_matmul* plan);
+
+/* lhs [m, k], rhs [n, k]: codes, 16-byte aligned with row strides that are multiples of 16 bytes;
+ * scales: any alignment and row stride; out: [m, n], aligned to its elements, any row stride (elements).
+ * m may be 0. Uses no workspace. */
+int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const void* lhs, int64_t lhs_row_stride,
+                                   const void* lhs_scales, int64_t lhs_scales_row_stride, const void* rhs,
+                                   int64_t rhs_row_stride, const void* rhs_scales, int64_t rhs_scales_row_stride,
+                                   void* out, int64_t out_row_stride, void* stream);
+
+/* Reads (and clears) the device status word; synchronises the stream first. */
+int32_t cake_scaled_matmul_status(cake_scaled_matmul* plan, void* stream, cake_status* out);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,215 @@
+"""The 8-bit linear layer without a GPU: the oracle's own arithmetic, plan refusals, C ABI refusals."""
+
+from __future__ import annotations
+
+import ctypes
+
+import ml_dtypes
+import numpy as np
+import pytest
+import torch
+
+from oracle import scaled as oracle
+from tpu_cake_b200 import _native
+from tpu_cake_b200 import scaled_cuda_lowering as scaled
+
+E4M3 = np.dtype(ml_dtypes.float8_e4m3fn)
+
+
+def test_oracle_rounds_like_the_format():
+    # Every e4m3 value rounds to itself, and the midpoints between neighbours go to the even code.
+    codes = np.arange(0x7F, dtype=np.uint8)
+    values = codes.view(E4M3).astype(np.float64)
+    assert np.array_equal(oracle.round_e4m3(values), values) and values[-1] == 448
+    middles = (values[:-1] + values[1:]) / 2
+    assert np.array_equal(oracle.round_e4m3(middles), values[codes[:-1] + (codes[:-1] & 1)])
+    generator = np.random.default_rng(0)
+    v = generator.uniform(-448, 448, 20000).astype(np.float32)
+    v[:5000] *= 2.0**-12
+    assert np.array_equal(oracle.round_e4m3(v.astype(np.float64)), v.astype(E4M3).astype(np.float64))
+
+
+@pytest.mark.parametrize("largest, scale", [(448.0, 1.0), (np.nextafter(448.0, 1e9), 2.0), (224.0, 0.5), (1e-45, 2.0**-127),
+                                            (0.0, 1.0), (3.4e38, 2.0**120), (np.inf, np.nan), (np.nan, np.nan)])
+def test_oracle_scale_is_the_least_power_of_two(largest, scale):
+    row = np.zeros((1, 130))
+    row[0, 7] = -largest if np.isfinite(largest) else largest
+    got = oracle.group_scales(row)
+    assert got.shape == (1, 2) and got[0, 1] == 1.0
+    assert np.isnan(got[0, 0]) if np.isnan(scale) else got[0, 0] == scale
+
+
+def test_plans_refuse_what_they_do_not_run():
+    for arguments in ({"columns": 0}, {"columns": 8, "input_dtype": "f64"}, {"columns": 8, "gate": "gelu"}):
+        with pytest.raises(ValueError):
+            scaled.CudaQuantizeRowsPlan(name="p", **arguments)
+    for arguments in ({"columns": 0}, {"columns": scaled.MAX_NORM_COLUMNS + 1}, {"columns": 8, "input_dtype": "i8"},
+                      {"columns": 8, "input_dtype": "bf16", "weight_dtype": "f16"}, {"columns": 8, "epsilon": -1.0},
+                      {"columns": 8, "epsilon": float("nan")}):
+        with pytest.raises(ValueError):
+            scaled.CudaRmsNormQuantizePlan(name="p", **arguments)
+    for arguments in ({"n": 0, "k": 8}, {"n": 8, "k": 0}, {"n": 1 << 30, "k": 8}, {"n": 8, "k": 8, "output_dtype": "f16"},
+                      {"n": 8, "k": 8, "tile": 256}, {"n": 8, "k": 8, "k_split": 2}, {"n": 8, "k": 8, "tile": 128, "k_split": 2},
+                      {"n": 8, "k": 8, "tile": 16, "k_split": 9}):
+        with pytest.raises(ValueError):
+            scaled.CudaScaledMatmulPlan(name="p", **arguments)
+
+
+def test_plan_sources_tell_plans_apart():
+    a = scaled.CudaScaledMatmulPlan(name="p", n=256, k=512)
+    assert a.source_sha256() == scaled.CudaScaledMatmulPlan(name="p", n=256, k=512).source_sha256()
+    assert a.source_sha256() != scaled.CudaScaledMatmulPlan(name="p", n=256, k=512, output_dtype="f32").source_sha256()
+    assert "cake_scaled_matmul_sm100" in a.render_executable_source()
+    assert "cake_rms_norm_quantize_sm100" in scaled.CudaRmsNormQuantizePlan(name="p", columns=64).render_executable_source()
+    assert "cake_quantize_rows_sm100" in scaled.CudaQuantizeRowsPlan(name="p", columns=64).render_executable_source()
+
+
+@pytest.mark.parametrize("columns, pitch", [(1, 16), (16, 16), (100, 112), (128, 128), (1000, 1008)])
+def test_codes_get_the_pitch_the_matmul_wants(columns, pitch):
+    codes = scaled.empty_codes(3, columns, torch.device("cpu"))
+    assert tuple(codes.shape) == (3, columns) and codes.stride() == (pitch, 1) and codes.dtype == torch.float8_e4m3fn
+    assert tuple(scaled.empty_scales(3, columns, torch.device("cpu")).shape) == (3, -(-columns // 128))
+
+
+class _Recorder:
+    """An executable that records what would be enqueued instead of calling the library."""
+
+    device = torch.device("cpu")
+
+    def __init__(self):
+        self.calls = []
+
+    def quantize(self, *arguments):
+        self.calls.append(arguments)
+
+    rms_norm_quantize = enqueue = quantize
+
+
+def test_invoke_refuses_wrong_operands():
+    recorder = _Recorder()
+    plan = scaled.CudaQuantizeRowsPlan(name="p", columns=100)
+    x = torch.zeros(4, 100, dtype=torch.bfloat16)
+    for wrong in (x.float(), x[:, :99], x[0], x.t(), torch.zeros(4, 200, dtype=torch.bfloat16)[:, ::2], x[:1].expand(4, 100), None):
+        with pytest.raises(ValueError, match="x must"):
+            plan.invoke(recorder, wrong)
+    with pytest.raises(ValueError, match="codes must"):
+        plan.invoke(recorder, x, codes=torch.zeros(3, 100).to(torch.float8_e4m3fn))
+    with pytest.raises(ValueError, match="scales must"):
+        plan.invoke(recorder, x, scales=torch.zeros(4, 2).to(torch.float8_e8m0fnu))
+    gated = scaled.CudaQuantizeRowsPlan(name="p", columns=100, gate="silu")
+    with pytest.raises(ValueError, match="x must"):
+        gated.invoke(recorder, x)
+
+    norm = scaled.CudaRmsNormQuantizePlan(name="p", columns=100)
+    weight = torch.ones(100, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="residual"):
+        norm.invoke(recorder, x, weight)
+    with pytest.raises(ValueError, match="weight"):
+        norm.invoke(recorder, x, weight.float(), x)
+    with pytest.raises(ValueError, match="weight"):
+        norm.invoke(recorder, x, torch.ones(200, dtype=torch.bfloat16)[::2], x)
+    with pytest.raises(ValueError, match="residual must"):
+        norm.invoke(recorder, x, weight, x[:3])
+    plain = scaled.CudaRmsNormQuantizePlan(name="p", columns=100, with_residual=False)
+    with pytest.raises(ValueError, match="residual"):
+        plain.invoke(recorder, x, weight, x)
+    with pytest.raises(ValueError, match="residual_out"):
+        plain.invoke(recorder, x, weight, residual_out=x)
+
+    matmul = scaled.CudaScaledMatmulPlan(name="p", n=32, k=256)
+    codes, scales = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.ones(4, 2).to(torch.float8_e8m0fnu)
+    rhs, rhs_scales = torch.zeros(32, 256).to(torch.float8_e4m3fn), torch.ones(32, 2).to(torch.float8_e8m0fnu)
+    for wrong in ((codes[:, :255], scales, rhs, rhs_scales), (codes, scales[:3], rhs, rhs_scales), (codes, scales, rhs[:31], rhs_scales[:31]),
+                  (codes, scales, rhs, rhs_scales[:, :1]), (codes.view(torch.float8_e5m2), scales, rhs, rhs_scales),
+                  (codes, scales.view(torch.uint8), rhs, rhs_scales)):
+        with pytest.raises(ValueError):
+            matmul.invoke(recorder, *wrong)
+    with pytest.raises(ValueError, match="out must"):
+        matmul.invoke(recorder, codes, scales, rhs, rhs_scales, out=torch.zeros(4, 32))
+    assert not recorder.calls
+    assert tuple(matmul.invoke(recorder, codes, scales, rhs, rhs_scales).shape) == (4, 32) and len(recorder.calls) == 1
+
+
+def _quantize(**overrides):
+    arguments = dict(x=1 << 20, dtype=1, x_stride=128, gate=0, rows=2, cols=128, q=1 << 20, q_stride=128, scales=1 << 20, scales_stride=1, stream=None)
+    arguments.update(overrides)
+    return _native.load().cake_quantize_rows_enqueue(*arguments.values())
+
+
+@pytest.mark.parametrize("overrides, code, fragment", [
+    ({"cols": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "columns"),
+    ({"cols": 1 << 40}, _native.CAKE_ERR_INVALID_ARGUMENT, "columns"),
+    ({"rows": -1}, _native.CAKE_ERR_INVALID_ARGUMENT, "rows"),
+    ({"rows": 1 << 31}, _native.CAKE_ERR_INVALID_ARGUMENT, "rows"),
+    ({"dtype": 7}, _native.CAKE_ERR_INVALID_ARGUMENT, "dtype"),
+    ({"gate": 2}, _native.CAKE_ERR_INVALID_ARGUMENT, "gate"),
+    ({"x": None}, _native.CAKE_ERR_INVALID_ARGUMENT, "null"),
+    ({"scales": None}, _native.CAKE_ERR_INVALID_ARGUMENT, "null"),
+    ({"x": (1 << 20) + 1}, _native.CAKE_ERR_INVALID_ARGUMENT, "aligned"),
+    ({"x_stride": 127}, _native.CAKE_ERR_INVALID_ARGUMENT, "stride"),
+    ({"gate": 1}, _native.CAKE_ERR_INVALID_ARGUMENT, "stride"),
+    ({"q_stride": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "stride"),
+    ({"scales_stride": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "stride"),
+])
+def test_quantize_refuses_bad_arguments(overrides, code, fragment):
+    assert _quantize(**overrides) == code
+    assert fragment in _native.load().cake_last_error().decode()
+
+
+def test_no_rows_is_no_work():
+    assert _quantize(rows=0, x=None, q=None, scales=None) == _native.CAKE_OK
+    assert _norm(rows=0, x=None, weight=None, q=None, scales=None) == _native.CAKE_OK
+
+
+def _norm(**overrides):
+    arguments = dict(x=1 << 20, dtype=1, x_stride=128, residual=None, residual_stride=0, residual_out=None, residual_out_stride=0, weight=1 << 20,
+                     weight_dtype=1, epsilon=1e-5, rows=2, cols=128, q=1 << 20, q_stride=128, scales=1 << 20, scales_stride=1, stream=None)
+    arguments.update(overrides)
+    return _native.load().cake_rms_norm_quantize_enqueue(*arguments.values())
+
+
+@pytest.mark.parametrize("overrides, code, fragment", [
+    ({"cols": 0}, _native.CAKE_ERR_UNSUPPORTED, "columns"),
+    ({"cols": 32769}, _native.CAKE_ERR_UNSUPPORTED, "columns"),
+    ({"weight_dtype": 2}, _native.CAKE_ERR_UNSUPPORTED, "weight"),
+    ({"epsilon": -1.0}, _native.CAKE_ERR_INVALID_ARGUMENT, "epsilon"),
+    ({"epsilon": float("nan")}, _native.CAKE_ERR_INVALID_ARGUMENT, "epsilon"),
+    ({"dtype": 9, "weight_dtype": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "dtype"),
+    ({"weight": None}, _native.CAKE_ERR_INVALID_ARGUMENT, "null"),
+    ({"weight": (1 << 20) + 1}, _native.CAKE_ERR_INVALID_ARGUMENT, "aligned"),
+    ({"residual": 1 << 20}, _native.CAKE_ERR_INVALID_ARGUMENT, "come together"),
+    ({"residual_out": 1 << 20}, _native.CAKE_ERR_INVALID_ARGUMENT, "come together"),
+    ({"residual": 1 << 20, "residual_out": 1 << 20, "residual_stride": 128}, _native.CAKE_ERR_INVALID_ARGUMENT, "stride"),
+    ({"x_stride": 5}, _native.CAKE_ERR_INVALID_ARGUMENT, "stride"),
+])
+def test_norm_refuses_bad_arguments(overrides, code, fragment):
+    assert _norm(**overrides) == code
+    assert fragment in _native.load().cake_last_error().decode()
+
+
+@pytest.mark.parametrize("overrides, code, fragment", [
+    ({"n": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
+    ({"k": 1 << 31}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
+    ({"out_dtype": 2}, _native.CAKE_ERR_INVALID_ARGUMENT, "out_dtype"),
+    ({"tile": 256}, _native.CAKE_ERR_UNSUPPORTED, "tile"),
+    ({"k_split": 9, "tile": 16}, _native.CAKE_ERR_INVALID_ARGUMENT, "k_split"),
+    ({"k_split": 2}, _native.CAKE_ERR_INVALID_ARGUMENT, "k_split"),
+    ({"k_split": 2, "tile": 224}, _native.CAKE_ERR_INVALID_ARGUMENT, "k_split"),
+    ({"reserved": 1}, _native.CAKE_ERR_INVALID_ARGUMENT, "reserved"),
+])
+def test_scaled_matmul_refuses_bad_descriptors(overrides, code, fragment):
+    lib = _native.load()
+    fields = dict(n=128, k=128, out_dtype=1, tile=0, k_split=0, reserved=0)
+    fields.update(overrides)
+    handle = ctypes.c_void_p()
+    assert lib.cake_scaled_matmul_create(ctypes.byref(_native.ScaledMatmulDesc(**fields)), ctypes.byref(handle)) == code
+    assert fragment in lib.cake_last_error().decode()
+
+
+def test_null_handles_are_errors_not_crashes():
+    lib = _native.load()
+    assert ctypes.sizeof(_native.ScaledMatmulDesc) == 32
+    assert lib.cake_scaled_matmul_create(None, None) == _native.CAKE_ERR_INVALID_ARGUMENT
+    assert lib.cake_scaled_matmul_enqueue(None, 1, None, 0, None, 0, None, 0, None, 0, None, 0, None) == _native.CAKE_ERR_INVALID_ARGUMENT
+    assert lib.cake_scaled_matmul_status(None, None, None) == _native.CAKE_ERR_INVALID_ARGUMENT
+    assert lib.cake_scaled_matmul_destroy(None) == _native.CAKE_OK

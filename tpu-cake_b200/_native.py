@@ -24,6 +24,9 @@ CAKE_ERR_STATE = -6
 
 CAKE_DTYPE_F32 = 0
 CAKE_DTYPE_BF16 = 1
+CAKE_DTYPE_F16 = 2
+CAKE_GATE_NONE = 0
+CAKE_GATE_SILU = 1
 CAKE_RS_LOCAL_PARTIAL = 0
 CAKE_RS_P2P_OWNER_PUSH = 1
 CAKE_RPA_CACHE_SEPARATE = 0
@@ -61,6 +64,12 @@ EXPORTED_SYMBOLS = (
     "cake_rpa_decode_static_scratch",
     "cake_rpa_status",
     "cake_rpa_launches_per_enqueue",
+    "cake_quantize_rows_enqueue",
+    "cake_rms_norm_quantize_enqueue",
+    "cake_scaled_matmul_create",
+    "cake_scaled_matmul_destroy",
+    "cake_scaled_matmul_enqueue",
+    "cake_scaled_matmul_status",
 )
 
 
@@ -119,6 +128,17 @@ class RpaDesc(ctypes.Structure):
         ("update_cache", ctypes.c_int32),
         ("kv_chunk_tokens", ctypes.c_int32),
         ("wait_budget_ms", ctypes.c_int32),
+    ]
+
+
+class ScaledMatmulDesc(ctypes.Structure):
+    _fields_ = [
+        ("n", ctypes.c_int64),
+        ("k", ctypes.c_int64),
+        ("out_dtype", ctypes.c_int32),
+        ("tile", ctypes.c_int32),
+        ("k_split", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -200,6 +220,20 @@ def load() -> ctypes.CDLL:
     lib.cake_rpa_status.argtypes = [vp, vp, ctypes.POINTER(CakeStatus)]
     lib.cake_rpa_launches_per_enqueue.restype = i32
     lib.cake_rpa_launches_per_enqueue.argtypes = [vp]
+
+    i64 = ctypes.c_int64
+    lib.cake_quantize_rows_enqueue.restype = i32
+    lib.cake_quantize_rows_enqueue.argtypes = [vp, i32, i64, i32, i64, i64, vp, i64, vp, i64, vp]
+    lib.cake_rms_norm_quantize_enqueue.restype = i32
+    lib.cake_rms_norm_quantize_enqueue.argtypes = [vp, i32, i64, vp, i64, vp, i64, vp, i32, ctypes.c_float, i64, i64, vp, i64, vp, i64, vp]
+    lib.cake_scaled_matmul_create.restype = i32
+    lib.cake_scaled_matmul_create.argtypes = [ctypes.POINTER(ScaledMatmulDesc), ctypes.POINTER(vp)]
+    lib.cake_scaled_matmul_destroy.restype = i32
+    lib.cake_scaled_matmul_destroy.argtypes = [vp]
+    lib.cake_scaled_matmul_enqueue.restype = i32
+    lib.cake_scaled_matmul_enqueue.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp]
+    lib.cake_scaled_matmul_status.restype = i32
+    lib.cake_scaled_matmul_status.argtypes = [vp, vp, ctypes.POINTER(CakeStatus)]
     _lib = lib
     return lib
 

@@ -12,7 +12,7 @@ PACKAGE_DIR = Path(__file__).resolve().parent
 CSRC = PACKAGE_DIR / "csrc"
 LIB_DIR = PACKAGE_DIR / "lib"
 LIBRARY = LIB_DIR / "libcake_b200.so"
-SOURCES = ("cake_runtime.cu", "matmul_rs_sm100.cu", "rpa_decode_sm100.cu")
+SOURCES = ("cake_runtime.cu", "matmul_rs_sm100.cu", "rpa_decode_sm100.cu", "row_quantize_sm100.cu", "scaled_matmul_sm100.cu")
 NVCC_FLAGS = (
     "-gencode",
     "arch=compute_100a,code=sm_100a",

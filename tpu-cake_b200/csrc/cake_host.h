@@ -35,6 +35,11 @@ int32_t encode_tensor_map_typed(CUtensorMap* out, const void* base, uint32_t ran
                                 const uint64_t* strides_bytes, const uint32_t* box, bool swizzle128,
                                 int elem_bytes);
 
+// Same, with the element type and the swizzle given.
+int32_t encode_tensor_map_as(CUtensorMap* out, const void* base, uint32_t rank, const uint64_t* dims,
+                             const uint64_t* strides_bytes, const uint32_t* box, CUtensorMapSwizzle swizzle,
+                             CUtensorMapDataType type);
+
 // Device status word helpers (4 x int32 in device memory).
 struct StatusWord {
   int32_t* dev = nullptr;

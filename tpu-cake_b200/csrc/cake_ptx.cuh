@@ -189,6 +189,18 @@ __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)
       : "memory");
 }
 
+// Same, 16 columns.
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+
 // Warp-collective: lane i writes 32 consecutive 32-bit columns of TMEM lane (base lane + i).
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t (&r)[32]) {
   asm volatile(
@@ -233,6 +245,66 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16_f32(uint32_t m, uint32_t 
                                                            uint32_t b_mn_major) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (a_mn_major << 15) | (b_mn_major << 16) |
          ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+
+// ----------------------------------------------------------------------------- tcgen05, 8-bit block scales
+
+// D[tmem] (+)= (A[smem] * scale A) * (B[smem] * scale B)^T for 8-bit operands, 32 deep, f32 accumulate;
+// issued by ONE thread. The scales are e8m0 bytes in tensor memory, one per operand row and 32 k: row r
+// of an operand has its 32-bit cell at lane r % 32 (repeated in all four lane quarters), column r / 32,
+// and the instruction descriptor names the byte of the cell.
+__device__ __forceinline__ void tcgen05_mma_mxf8(uint32_t tmem_d, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                 uint32_t tmem_sfa, uint32_t tmem_sfb, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t"
+      "}\n"
+      ::"r"(tmem_d), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(tmem_sfa), "r"(tmem_sfb), "r"(accumulate)
+      : "memory");
+}
+
+// Copies 32 rows of 16 bytes from shared memory to four 32-bit tensor-memory columns, the same in all
+// four lane quarters (how the scales above are brought in). Ordered before later MMAs of this thread.
+__device__ __forceinline__ void tcgen05_cp_32x128b_warpx4(uint32_t tmem_dst, uint64_t s_desc) {
+  asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(tmem_dst), "l"(s_desc) : "memory");
+}
+
+// Shared-memory descriptor of such a block: no swizzle, groups of eight 16-byte rows 128 bytes apart.
+__device__ __forceinline__ uint64_t umma_desc_scales(uint32_t smem_addr) {
+  return static_cast<uint64_t>((smem_addr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(128 >> 4) << 32) | (1ull << 46);
+}
+
+// Instruction descriptor for kind::mxf8f6f4 with e4m3 A and B (format 0, both K-major) and e8m0 scales
+// (bit 23): N >> 3 at [17,23), M >> 4 at [24,29); scale byte of B at [4,6) and of A at [29,31).
+__host__ __device__ constexpr uint32_t umma_idesc_mxf8(uint32_t m, uint32_t n, uint32_t scale_byte) {
+  return (scale_byte << 4) | ((n >> 3) << 17) | (1u << 23) | ((m >> 4) << 24) | (scale_byte << 29);
+}
+
+// ----------------------------------------------------------------------------- thread-block clusters
+
+__device__ __forceinline__ uint32_t cluster_cta_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+
+// Every thread of every block of the cluster: what was written to shared memory before is visible after.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Four f32 from the shared memory of the cluster's block `rank`, at the place `smem_addr` has in this block's.
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t smem_addr, uint32_t rank) {
+  uint32_t remote;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(smem_addr), "r"(rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(remote)
+               : "memory");
+  return v;
 }
 
 // ----------------------------------------------------------------------------- system-scope flags

@@ -1,0 +1,744 @@
+// Block-scaled 8-bit matmul for sm_100a: out[m, n] = sum over k of
+// (lhs[m, k] 2^(sl[m, k / 128] - 127)) * (rhs[n, k] 2^(sr[n, k / 128] - 127)), e4m3 codes, e8m0 scales, f32
+// accumulation in tensor memory, one rounding to the output type.
+//
+// The scales are powers of two, so the tensor core applies them itself (kind::mxf8f6f4, one scale per
+// operand row and 32 k; the four 32-deep steps of a 128-deep block name the same byte): nothing is
+// multiplied in the epilogue and no partial sum leaves tensor memory before the end of the contraction.
+// With scales of any mantissa every 128-deep block's 128 x N products would have to be read back, scaled
+// and added in registers.
+//
+// One kernel template, two shapes of work. "A" is the 128-row operand of an MMA, "B" the one of BN rows.
+//   wide    A = lhs, B = rhs: 128 x BN output tiles, persistent blocks, two accumulators, so that a
+//           tile's epilogue runs under the next one's main loop.
+//   narrow  A = rhs, B = lhs: 128 columns of the output by BN tokens. Few tokens: bound by reading rhs
+//           once, so BN is as small as the tokens allow, and the contraction of a tile is split over the
+//           blocks of a cluster, which add their partial sums through distributed shared memory in rank
+//           order (no workspace, no atomics: the same bits every time).
+// Warps: 0 TMA producer (128-byte swizzled rows of 128 codes, one k block per stage), 1 MMA issue and
+// tensor memory, 2 scales, 4-7 epilogue. The scales warp gathers a 32-bit word -- four k blocks' bytes --
+// per operand row, so that scales are taken as they lie, with any stride, and puts them into shared memory
+// in the order tcgen05.cp wants: lane i's 16 bytes are rows i, 32 + i, 64 + i, 96 + i.
+#include <cuda_bf16.h>
+#include <string.h>
+
+#include <new>
+
+#include "cake_host.h"
+#include "cake_ptx.cuh"
+
+namespace cake {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kRowsA = 128;
+constexpr int kBlockK = 128;  // codes (= bytes) of a k block: one swizzle row, one scale
+constexpr int kUmmaK = 32;
+constexpr int kScaleSlots = 4;          // shared-memory ring of scale words (four k blocks each)
+constexpr int kScaleSets = 2;           // sets of scale columns in tensor memory, used in turn
+constexpr int kStagingSlots = 2;        // 32 x 32 output chunks an epilogue warp may have in flight
+constexpr uint32_t kStagingBytes = 32 * 128;
+constexpr int kReducePitch = kRowsA + 4;  // floats between two tokens' partial sums
+constexpr long long kBudgetCycles = 4000000000ll;  // about two seconds of SM clock
+
+constexpr int pow2_at_least(int v) {
+  int p = 32;
+  while (p < v) p *= 2;
+  return p;
+}
+
+template <int BN, bool NARROW>
+struct Cfg {
+  static constexpr uint32_t kABytes = kRowsA * kBlockK;
+  static constexpr uint32_t kStageBytes = kABytes + BN * kBlockK;
+  static constexpr int kScaleBlocksB = (BN + 127) / 128;
+  static constexpr uint32_t kScaleSlotBytes = 512 * (1 + kScaleBlocksB);
+  static constexpr uint32_t kStaging = NARROW ? 0 : 4 * kStagingSlots * kStagingBytes;
+  // Narrow: two blocks share an SM. Wide: one block has it all.
+  static constexpr uint32_t kRoom = (NARROW ? 112 * 1024 : 226 * 1024) - 1024 /*alignment*/ - 512 /*barriers*/;
+  static constexpr int kFit = static_cast<int>((kRoom - kStaging - kScaleSlots * kScaleSlotBytes) / kStageBytes);
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
+  // Accumulators, then kScaleSets sets of scale columns (4 for A, 4 per 128 rows of B).
+  static constexpr int kAccumulators = NARROW ? 1 : 2;
+  static constexpr int kScaleCols = 4 * (1 + kScaleBlocksB);
+  static constexpr int kScaleBase = kAccumulators * BN;
+  static constexpr int kTmemCols = pow2_at_least(kScaleBase + kScaleSets * kScaleCols);
+  static_assert(kTmemCols <= (NARROW ? 256 : 512), "tensor memory of an SM");
+  static constexpr uint32_t kSmemBytes = kStages * kStageBytes + kStaging + kScaleSlots * kScaleSlotBytes + 512 + 1024;
+  static_assert(!NARROW || BN * kReducePitch * 4 <= kStages * kStageBytes, "partial sums take the operand ring's place");
+};
+
+struct Params {
+  int32_t rows_a, rows_b;    // rows of the two operands (wide: m and n; narrow: n and m)
+  int32_t tiles_a, tiles_b;
+  int32_t k, k_blocks;
+  int32_t split;             // blocks of a cluster that share a tile (narrow)
+  int32_t out_f32, tma_store;
+  const uint8_t* scales_a;
+  const uint8_t* scales_b;
+  int64_t scales_a_stride, scales_b_stride;
+  void* out;
+  int64_t out_stride;
+  int32_t* status;
+};
+
+__device__ __forceinline__ void record(int32_t* status, int code, int d0, int d1, int d2) {
+  if (status && atomicCAS(status, 0, code) == 0) {
+    status[1] = d0;
+    status[2] = d1;
+    status[3] = d2;
+  }
+}
+
+// Bounded wait that also gives up when another role of this block has.
+__device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (clock64() - start > kBudgetCycles) return false;
+  }
+}
+
+// Four k blocks' scale bytes of one operand row, from k block kb on; 127 (the number 1) past the row's
+// end and for rows past the operand's, where all codes are zero. ALIGNED: base and stride are multiples
+// of four, and so is kb.
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* scales, int64_t stride, int row, int rows, int kb, int k_blocks, bool aligned) {
+  if (row >= rows) return 0x7F7F7F7Fu;
+  const uint8_t* src = scales + static_cast<int64_t>(row) * stride + kb;
+  if (aligned && kb + 4 <= k_blocks) return __ldg(reinterpret_cast<const uint32_t*>(src));
+  uint32_t w = 0x7F7F7F7Fu;
+  for (int i = 0; i < 4; ++i)
+    if (kb + i < k_blocks) w = (w & ~(0xFFu << (8 * i))) | (static_cast<uint32_t>(src[i]) << (8 * i));
+  return w;
+}
+
+// Consecutive tiles walk 16 row tiles down before moving one column tile right, so that the blocks of a
+// wave share both operands' rows in L2.
+__device__ __forceinline__ void raster(int t, int tiles_a, int tiles_b, int& ta, int& tb) {
+  const int group = 16 * tiles_b;
+  const int g = t / group;
+  const int rows = min(16, tiles_a - g * 16);
+  const int r = t - g * group;
+  ta = g * 16 + r % rows;
+  tb = r / rows;
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int BN, bool NARROW>
+__global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
+    cake_scaled_matmul_sm100(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                             const __grid_constant__ CUtensorMap map_out, const __grid_constant__ Params p) {
+  using C = Cfg<BN, NARROW>;
+  constexpr int STAGES = C::kStages;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint8_t* staging = smem + STAGES * C::kStageBytes;
+  uint8_t* scale_ring = staging + C::kStaging;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(scale_ring + kScaleSlots * C::kScaleSlotBytes);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = full_bar + STAGES;
+  uint64_t* scale_full = empty_bar + STAGES;
+  uint64_t* scale_empty = scale_full + kScaleSlots;
+  uint64_t* tmem_full = scale_empty + kScaleSlots;
+  uint64_t* tmem_empty = tmem_full + 2;
+  uint64_t* drain_bar = tmem_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  volatile uint32_t* abort_flag = tmem_slot + 1;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const int num_tiles = p.tiles_a * p.tiles_b;
+  // Narrow: one tile per cluster, this block's share of its k blocks. Wide: tiles by stride, all k blocks.
+  const int rank = NARROW ? static_cast<int>(blockIdx.x) % p.split : 0;
+  const int first_tile = NARROW ? static_cast<int>(blockIdx.x) / p.split : static_cast<int>(blockIdx.x);
+  const int tile_step = NARROW ? num_tiles : static_cast<int>(gridDim.x);
+  const int kb_begin = NARROW ? static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / p.split) : 0;
+  const int kb_end = NARROW ? static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / p.split) : p.k_blocks;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), 1);
+    }
+    for (int s = 0; s < kScaleSlots; ++s) {
+      mbar_init(smem_u32(&scale_full[s]), 1);
+      mbar_init(smem_u32(&scale_empty[s]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&tmem_full[b]), 1);
+      mbar_init(smem_u32(&tmem_empty[b]), 4);
+    }
+    mbar_init(smem_u32(drain_bar), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+    prefetch_tensormap(&map_a);
+    prefetch_tensormap(&map_b);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+    tmem_relinquish();
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  grid_dependency_wait();
+  grid_dependency_trigger();
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
+        int ta, tb;
+        raster(t, p.tiles_a, p.tiles_b, ta, tb);
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+          if (!wait_or_abort(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag)) {
+            if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 100 + stage);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t full = smem_u32(&full_bar[stage]);
+          const uint32_t dst = smem_u32(smem + stage * C::kStageBytes);
+          mbar_arrive_expect_tx(full, C::kStageBytes);
+          tma_load_2d(dst, &map_a, full, kb * kBlockK, ta * kRowsA);
+          tma_load_2d(dst + C::kABytes, &map_b, full, kb * kBlockK, tb * BN);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        // Let copies in flight land before the block's shared memory is released.
+        for (int s = 0; s < STAGES; ++s)
+          mbar_wait_bounded(smem_u32(&full_bar[s]), s < stage ? phase : (phase ^ 1), 200000000ll);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA issue
+    if (lane == 0) {
+      int stage = 0, it = 0;
+      uint32_t phase = 0;
+      uint32_t words = 0;  // scale words (four k blocks each) brought in so far
+      bool ok = true;
+      for (int t = first_tile; t < num_tiles && ok; t += tile_step, ++it) {
+        const int buf = C::kAccumulators == 2 ? (it & 1) : 0;
+        const uint32_t acc_phase = C::kAccumulators == 2 ? ((it >> 1) & 1) : (it & 1);
+        if (!wait_or_abort(smem_u32(&tmem_empty[buf]), acc_phase ^ 1, abort_flag)) {
+          if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 200 + buf);
+          *abort_flag = 1;
+          break;
+        }
+        tcgen05_fence_after();
+        const uint32_t tmem_d = tmem_base + buf * BN;
+        uint32_t sfa = 0;
+        for (int kb = kb_begin; kb < kb_end; ++kb) {
+          const uint32_t byte = static_cast<uint32_t>(kb - kb_begin) & 3u;
+          const uint32_t slot = words % kScaleSlots;
+          if (byte == 0) {
+            // The set of scale columns was last used kScaleSets words ago: the MMAs of that word, whose
+            // completion also freed its slot of the ring, must be done.
+            if (words >= kScaleSets) {
+              const uint32_t old = words - kScaleSets;
+              ok = wait_or_abort(smem_u32(&scale_empty[old % kScaleSlots]), (old / kScaleSlots) & 1, abort_flag);
+            }
+            if (!ok || !wait_or_abort(smem_u32(&scale_full[slot]), (words / kScaleSlots) & 1, abort_flag)) {
+              if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 500 + slot);
+              *abort_flag = 1;
+              ok = false;
+              break;
+            }
+            tcgen05_fence_after();
+            const uint32_t src = smem_u32(scale_ring + slot * C::kScaleSlotBytes);
+            sfa = tmem_base + C::kScaleBase + (words % kScaleSets) * C::kScaleCols;
+            tcgen05_cp_32x128b_warpx4(sfa, umma_desc_scales(src));
+#pragma unroll
+            for (int b = 0; b < C::kScaleBlocksB; ++b)
+              tcgen05_cp_32x128b_warpx4(sfa + 4 + 4 * b, umma_desc_scales(src + 512 * (1 + b)));
+          }
+          if (!wait_or_abort(smem_u32(&full_bar[stage]), phase, abort_flag)) {
+            if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 300 + stage);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const uint32_t a_addr = smem_u32(smem + stage * C::kStageBytes);
+          const uint32_t b_addr = a_addr + C::kABytes;
+          const uint32_t idesc = umma_idesc_mxf8(kRowsA, BN, 0) | (byte << 4) | (byte << 29);
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / kUmmaK; ++kk) {
+            // K-major rows of 128 bytes, groups of eight 1024 bytes apart; a step of 32 codes is 32 bytes
+            // inside the swizzle row.
+            tcgen05_mma_mxf8(tmem_d, umma_desc_sw128(a_addr + kk * kUmmaK, 16, 1024), umma_desc_sw128(b_addr + kk * kUmmaK, 16, 1024),
+                             idesc, sfa, sfa + 4, kb != kb_begin || kk != 0 ? 1u : 0u);
+          }
+          tcgen05_commit(smem_u32(&empty_bar[stage]));
+          if (byte == 3 || kb == kb_end - 1) {
+            tcgen05_commit(smem_u32(&scale_empty[slot]));
+            ++words;
+          }
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok) tcgen05_commit(smem_u32(&tmem_full[buf]));
+      }
+      // Everything issued above has retired before tensor memory is released.
+      tcgen05_commit(smem_u32(drain_bar));
+      mbar_wait_bounded(smem_u32(drain_bar), 0, kBudgetCycles);
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------------ scales
+    const bool aligned_a = ((reinterpret_cast<uintptr_t>(p.scales_a) | static_cast<uintptr_t>(p.scales_a_stride)) & 3) == 0 && (kb_begin & 3) == 0;
+    const bool aligned_b = ((reinterpret_cast<uintptr_t>(p.scales_b) | static_cast<uintptr_t>(p.scales_b_stride)) & 3) == 0 && (kb_begin & 3) == 0;
+    constexpr int kBlocks = 1 + C::kScaleBlocksB;
+    uint32_t next[kBlocks][4];
+    auto fetch = [&](int ta, int tb, int kb) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        next[0][c] = scale_word(p.scales_a, p.scales_a_stride, ta * kRowsA + c * 32 + lane, p.rows_a, kb, p.k_blocks, aligned_a);
+#pragma unroll
+      for (int b = 1; b < kBlocks; ++b)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const int r = (b - 1) * 128 + c * 32;  // of the tile's BN rows; a BN below 32 has lanes past it
+          next[b][c] = r + lane < BN ? scale_word(p.scales_b, p.scales_b_stride, tb * BN + r + lane, p.rows_b, kb, p.k_blocks, aligned_b) : 0x7F7F7F7Fu;
+        }
+    };
+    int slot = 0;
+    uint32_t slot_phase = 0;
+    int t = first_tile, kb = kb_begin, ta = 0, tb = 0;
+    if (t < num_tiles) {
+      raster(t, p.tiles_a, p.tiles_b, ta, tb);
+      fetch(ta, tb, kb);
+    }
+    while (t < num_tiles) {
+      uint32_t now[kBlocks][4];
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) now[b][c] = next[b][c];
+      // The next words are on their way while this slot is waited for.
+      kb += 4;
+      if (kb >= kb_end) {
+        t += tile_step;
+        kb = kb_begin;
+        if (t < num_tiles) raster(t, p.tiles_a, p.tiles_b, ta, tb);
+      }
+      if (t < num_tiles) fetch(ta, tb, kb);
+      if (!__all_sync(0xffffffffu, wait_or_abort(smem_u32(&scale_empty[slot]), slot_phase ^ 1, abort_flag))) {
+        if (!*abort_flag && lane == 0) record(p.status, 1, blockIdx.x, t, 600 + slot);
+        *abort_flag = 1;
+        break;
+      }
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+        *reinterpret_cast<uint4*>(scale_ring + slot * C::kScaleSlotBytes + b * 512 + lane * 16) =
+            make_uint4(now[b][0], now[b][1], now[b][2], now[b][3]);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&scale_full[slot]));
+      if (++slot == kScaleSlots) {
+        slot = 0;
+        slot_phase ^= 1;
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------------ epilogue
+    const int q = warp & 3;  // the lane quarter of tensor memory this warp may read
+    uint8_t* my_staging = staging + q * kStagingSlots * kStagingBytes;
+    int staged = 0, it = 0;
+    for (int t = first_tile; t < num_tiles; t += tile_step, ++it) {
+      int ta, tb;
+      raster(t, p.tiles_a, p.tiles_b, ta, tb);
+      const int buf = C::kAccumulators == 2 ? (it & 1) : 0;
+      const uint32_t acc_phase = C::kAccumulators == 2 ? ((it >> 1) & 1) : (it & 1);
+      // Warp-uniform: tcgen05.ld is a warp's instruction.
+      if (!__all_sync(0xffffffffu, wait_or_abort(smem_u32(&tmem_full[buf]), acc_phase, abort_flag))) {
+        if (!*abort_flag && lane == 0) record(p.status, 1, blockIdx.x, t, 400 + buf);
+        *abort_flag = 1;
+        break;
+      }
+      tcgen05_fence_after();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
+      const int row0 = ta * kRowsA + q * 32;
+      if (NARROW) {
+        // Lane = output column, register = token. Alone, the block stores 32 columns of a token at a
+        // time; sharing the tile, it leaves its partial sums in the operand ring, which is free: the
+        // last MMA has read it.
+        const int tokens = min(BN, p.rows_b - tb * BN);
+        float* partial = reinterpret_cast<float*>(smem);
+        const int col = row0 + lane;
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 16) {
+          if (c >= tokens) break;
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(t_row + c, v);
+          tmem_ld_wait();
+          if (p.split > 1) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) partial[(c + j) * kReducePitch + q * 32 + lane] = __uint_as_float(v[j]);
+          } else if (col < p.rows_a) {
+            const int64_t at = static_cast<int64_t>(tb * BN + c) * p.out_stride + col;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (c + j < tokens) {
+                if (p.out_f32) static_cast<float*>(p.out)[at + j * p.out_stride] = __uint_as_float(v[j]);
+                else static_cast<__nv_bfloat16*>(p.out)[at + j * p.out_stride] = __float2bfloat16_rn(__uint_as_float(v[j]));
+              }
+            }
+          }
+        }
+        tcgen05_fence_before();
+        continue;
+      }
+      // Wide: lane = output row, register = column. Chunks of 32 x 32 leave through shared memory, in the
+      // layout of a swizzled tensor store's box (64-byte rows of bf16, 128-byte rows of f32).
+      const int row_bytes = p.out_f32 ? 128 : 64;
+#pragma unroll 1
+      for (int c = 0; c < BN; c += 32) {
+        uint32_t v[32];
+        tmem_ld_32x32b_x32(t_row + c, v);
+        tmem_ld_wait();
+        if (c == BN - 32) {
+          tcgen05_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&tmem_empty[buf]));
+        }
+        const int col = tb * BN + c;
+        if (row0 >= p.rows_a || col >= p.rows_b) continue;  // warp-uniform
+        uint8_t* slot = my_staging + (staged % kStagingSlots) * kStagingBytes;
+        if (p.tma_store && staged >= kStagingSlots) {
+          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStagingSlots - 1) : "memory");
+          __syncwarp();
+        }
+        ++staged;
+        if (p.out_f32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            *reinterpret_cast<uint4*>(slot + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(v[8 * j + 2 * e]), __uint_as_float(v[8 * j + 2 * e + 1]));
+            *reinterpret_cast<uint4*>(slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        if (p.tma_store) {
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                         ::"l"(reinterpret_cast<uint64_t>(&map_out)), "r"(smem_u32(slot)), "r"(col), "r"(row0)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          }
+          continue;
+        }
+        // Rows whose pitch or base is not a multiple of 16 bytes: one row of 32 columns per store.
+        __syncwarp();
+        if (col + lane < p.rows_b) {
+          const int rows = min(32, p.rows_a - row0);
+          for (int r = 0; r < rows; ++r) {
+            const int64_t at = static_cast<int64_t>(row0 + r) * p.out_stride + col + lane;
+            if (p.out_f32) {
+              static_cast<float*>(p.out)[at] = *reinterpret_cast<const float*>(slot + r * row_bytes + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
+            } else {
+              static_cast<__nv_bfloat16*>(p.out)[at] =
+                  *reinterpret_cast<const __nv_bfloat16*>(slot + r * row_bytes + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+    // Shared memory outlives every tensor store that still reads it.
+    if (!NARROW && p.tma_store && lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+  __syncwarp();
+
+  if (NARROW && p.split > 1) {
+    // Every block of the cluster takes its share of the tile's (token, four columns) pieces and adds the
+    // partial sums of all blocks in rank order.
+    cluster_sync();
+    int ta, tb;
+    raster(first_tile, p.tiles_a, p.tiles_b, ta, tb);
+    const int tokens = min(BN, p.rows_b - tb * BN);
+    const int pieces = tokens * (kRowsA / 4);
+    if (!*abort_flag) {
+      for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < pieces; i += p.split * kThreads) {
+        const int token = i / (kRowsA / 4), c4 = (i % (kRowsA / 4)) * 4;
+        const uint32_t at = smem_u32(smem) + (token * kReducePitch + c4) * 4;
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int s = 0; s < p.split; ++s) {
+          const float4 v = ld_cluster_f32x4(at, s);
+          sum.x += v.x;
+          sum.y += v.y;
+          sum.z += v.z;
+          sum.w += v.w;
+        }
+        const float e[4] = {sum.x, sum.y, sum.z, sum.w};
+        const int col = ta * kRowsA + c4;
+        const int64_t dst = static_cast<int64_t>(tb * BN + token) * p.out_stride + col;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if (col + j < p.rows_a) {
+            if (p.out_f32) static_cast<float*>(p.out)[dst + j] = e[j];
+            else static_cast<__nv_bfloat16*>(p.out)[dst + j] = __float2bfloat16_rn(e[j]);
+          }
+        }
+      }
+    }
+    __syncwarp();
+    cluster_sync();  // no block leaves while another reads its shared memory
+  }
+  tcgen05_fence_before();
+  __syncthreads();
+  tcgen05_fence_after();
+  if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
+}
+
+}  // namespace
+}  // namespace cake
+
+// ====================================================================================== host
+
+struct cake_scaled_matmul {
+  cake_scaled_matmul_desc d;
+  int device = 0;
+  int sm_count = 0;
+  cake::StatusWord status;
+};
+
+namespace {
+
+using cake::fail;
+
+template <int BN, bool NARROW>
+int32_t launch(const cake_scaled_matmul* plan, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out,
+               const cake::Params& p, cudaStream_t stream) {
+  using C = cake::Cfg<BN, NARROW>;
+  auto kernel = cake::cake_scaled_matmul_sm100<BN, NARROW>;
+  // The opt-in to more than 48 KB of dynamic shared memory is a per-device attribute.
+  static bool configured[64] = {};
+  const int slot = plan->device >= 0 && plan->device < 64 ? plan->device : 0;
+  if (!configured[slot]) {
+    CAKE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
+    configured[slot] = plan->device >= 0 && plan->device < 64;
+  }
+  const int64_t tiles = static_cast<int64_t>(p.tiles_a) * p.tiles_b;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = NARROW ? p.split : 1;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(NARROW ? tiles * p.split : (tiles < plan->sm_count ? tiles : plan->sm_count)));
+  config.blockDim = dim3(cake::kThreads);
+  config.dynamicSmemBytes = C::kSmemBytes;
+  config.stream = stream;
+  config.attrs = attrs;
+  config.numAttrs = NARROW && p.split > 1 ? 2 : 1;
+  CAKE_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a, b, out, p));
+  return CAKE_OK;
+}
+
+int32_t encode_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t k, int64_t stride, int box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(k), static_cast<uint64_t>(rows)};
+  const uint64_t strides[1] = {static_cast<uint64_t>(stride)};
+  const uint32_t box[2] = {cake::kBlockK, static_cast<uint32_t>(box_rows)};
+  return cake::encode_tensor_map_as(map, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_UINT8);
+}
+
+// What a call runs: the tile, and for few tokens the blocks that share one.
+struct Choice {
+  int tile, split;
+};
+
+bool is_narrow(int tile) { return tile <= 64; }
+
+Choice choose(const cake_scaled_matmul* plan, int64_t m) {
+  const cake_scaled_matmul_desc& d = plan->d;
+  Choice c = {d.tile, d.k_split};
+  const int64_t k_blocks = (d.k + cake::kBlockK - 1) / cake::kBlockK;
+  if (c.tile == 0) {
+    if (m <= 16) c.tile = 16;
+    else if (m <= 32) c.tile = 32;
+    else if (m <= 256) c.tile = 64;
+    else {
+      int64_t best = 0;
+      for (int tile : {128, 192, 224}) {
+        const int64_t tiles = ((m + 127) / 128) * ((d.n + tile - 1) / tile);
+        const int64_t cost = (tiles + plan->sm_count - 1) / plan->sm_count * tile;
+        if (best == 0 || cost <= best) {
+          best = cost;
+          c.tile = tile;
+        }
+      }
+    }
+  }
+  if (!is_narrow(c.tile)) c.split = 1;
+  else if (c.split == 0) {
+    const int64_t tiles = ((d.n + 127) / 128) * ((m + c.tile - 1) / c.tile);
+    c.split = 1;
+    while (c.split < 8 && 2 * c.split * tiles <= plan->sm_count && 2 * c.split <= k_blocks) c.split *= 2;
+  }
+  if (c.split > k_blocks) c.split = static_cast<int>(k_blocks);
+  return c;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t cake_scaled_matmul_create(const cake_scaled_matmul_desc* desc, cake_scaled_matmul** out) {
+  if (!desc || !out) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_create: null argument");
+  const cake_scaled_matmul_desc& d = *desc;
+  // Rows and columns are tensor-map coordinates; a tile past the end must not wrap around either.
+  if (d.n < 1 || d.k < 1 || d.n > INT32_MAX / 2 || d.k > INT32_MAX / 2)
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "scaled matmul extents must be 1 to 2^30 - 1: n=%lld k=%lld", (long long)d.n, (long long)d.k);
+  if (d.out_dtype != CAKE_DTYPE_F32 && d.out_dtype != CAKE_DTYPE_BF16)
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "out_dtype must be CAKE_DTYPE_F32 or CAKE_DTYPE_BF16");
+  if (d.tile != 0 && d.tile != 16 && d.tile != 32 && d.tile != 64 && d.tile != 128 && d.tile != 192 && d.tile != 224)
+    return fail(CAKE_ERR_UNSUPPORTED, "tile must be 0, 16, 32, 64, 128, 192 or 224, got %d", d.tile);
+  if (d.k_split < 0 || d.k_split > 8 || (d.k_split > 1 && !is_narrow(d.tile)) || (d.k_split > 1 && d.tile == 0))
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "k_split must be 0 to 8, and above 1 only with tile 16, 32 or 64, got %d", d.k_split);
+  if (d.reserved != 0) return fail(CAKE_ERR_INVALID_ARGUMENT, "reserved must be 0");
+  cake_scaled_matmul* plan = new (std::nothrow) cake_scaled_matmul();
+  if (!plan) return fail(CAKE_ERR_CUDA, "out of host memory");
+  plan->d = d;
+  cudaError_t e = cudaGetDevice(&plan->device);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&plan->sm_count, cudaDevAttrMultiProcessorCount, plan->device);
+  int major = 0;
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, plan->device);
+  if (e != cudaSuccess) {
+    delete plan;
+    return fail(CAKE_ERR_CUDA, "no usable CUDA device: %s", cudaGetErrorString(e));
+  }
+  if (major != 10) {
+    delete plan;
+    return fail(CAKE_ERR_UNSUPPORTED, "libcake_b200 needs an sm_100 GPU, found compute capability %d.x", major);
+  }
+  const int32_t rc = plan->status.ensure();
+  if (rc != CAKE_OK) {
+    cake_scaled_matmul_destroy(plan);
+    return rc;
+  }
+  *out = plan;
+  return CAKE_OK;
+}
+
+int32_t cake_scaled_matmul_destroy(cake_scaled_matmul* plan) {
+  if (!plan) return CAKE_OK;
+  plan->status.release();
+  delete plan;
+  return CAKE_OK;
+}
+
+int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const void* lhs, int64_t lhs_row_stride,
+                                   const void* lhs_scales, int64_t lhs_scales_row_stride, const void* rhs,
+                                   int64_t rhs_row_stride, const void* rhs_scales, int64_t rhs_scales_row_stride,
+                                   void* out, int64_t out_row_stride, void* stream) {
+  if (!plan) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_enqueue: null argument");
+  const cake_scaled_matmul_desc& d = plan->d;
+  if (m < 0 || m > INT32_MAX / 2) return fail(CAKE_ERR_INVALID_ARGUMENT, "m must be 0 to 2^30 - 1, got %lld", (long long)m);
+  if (m == 0) return CAKE_OK;
+  if (!lhs || !lhs_scales || !rhs || !rhs_scales || !out) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_enqueue: null argument");
+  const int osize = d.out_dtype == CAKE_DTYPE_F32 ? 4 : 2;
+  const int64_t k_blocks = (d.k + cake::kBlockK - 1) / cake::kBlockK;
+  // With a single row its stride says nothing; tensor maps still want a valid one.
+  const int64_t pitch = (d.k + 15) / 16 * 16;
+  if (m == 1) {
+    lhs_row_stride = pitch;
+    out_row_stride = d.n;
+  }
+  if (d.n == 1) rhs_row_stride = pitch;
+  if ((reinterpret_cast<uintptr_t>(lhs) | reinterpret_cast<uintptr_t>(rhs)) & 15)
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "lhs and rhs must be 16-byte aligned");
+  if (lhs_row_stride % 16 || rhs_row_stride % 16 || lhs_row_stride < d.k || rhs_row_stride < d.k)
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "lhs and rhs row strides must be multiples of 16 bytes and at least k, got %lld and %lld",
+                (long long)lhs_row_stride, (long long)rhs_row_stride);
+  if ((m > 1 && lhs_scales_row_stride < k_blocks) || (d.n > 1 && rhs_scales_row_stride < k_blocks))
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "a scales row stride is shorter than its %lld scales", (long long)k_blocks);
+  if (out_row_stride < d.n) return fail(CAKE_ERR_INVALID_ARGUMENT, "the output row stride is shorter than its row");
+  if (reinterpret_cast<uintptr_t>(out) % osize) return fail(CAKE_ERR_INVALID_ARGUMENT, "out is not aligned to its elements");
+
+  const Choice c = choose(plan, m);
+  const bool narrow = is_narrow(c.tile);
+  cake::Params p;
+  memset(&p, 0, sizeof(p));
+  const int64_t rows_a = narrow ? d.n : m, rows_b = narrow ? m : d.n;
+  p.rows_a = static_cast<int32_t>(rows_a);
+  p.rows_b = static_cast<int32_t>(rows_b);
+  const int64_t tiles_a = (rows_a + cake::kRowsA - 1) / cake::kRowsA, tiles_b = (rows_b + c.tile - 1) / c.tile;
+  if (tiles_a * tiles_b * c.split > INT32_MAX / 2)
+    return fail(CAKE_ERR_UNSUPPORTED, "%lld x %lld tiles are more than one launch covers", (long long)tiles_a, (long long)tiles_b);
+  p.tiles_a = static_cast<int32_t>(tiles_a);
+  p.tiles_b = static_cast<int32_t>(tiles_b);
+  p.k = static_cast<int32_t>(d.k);
+  p.k_blocks = static_cast<int32_t>(k_blocks);
+  p.split = c.split;
+  p.out_f32 = osize == 4;
+  p.scales_a = static_cast<const uint8_t*>(narrow ? rhs_scales : lhs_scales);
+  p.scales_b = static_cast<const uint8_t*>(narrow ? lhs_scales : rhs_scales);
+  p.scales_a_stride = narrow ? rhs_scales_row_stride : lhs_scales_row_stride;
+  p.scales_b_stride = narrow ? lhs_scales_row_stride : rhs_scales_row_stride;
+  p.out = out;
+  p.out_stride = out_row_stride;
+  p.status = plan->status.dev;
+  // Tensor stores write whole 16-byte pieces, also where the row ends inside one: only rows of whole pieces
+  // leave what lies behind them alone.
+  p.tma_store = !narrow && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && out_row_stride * osize % 16 == 0 && d.n * osize % 16 == 0;
+
+  CUtensorMap map_a, map_b, map_out;
+  memset(&map_out, 0, sizeof(map_out));
+  int32_t rc = encode_operand(&map_a, narrow ? rhs : lhs, rows_a, d.k, narrow ? rhs_row_stride : lhs_row_stride, cake::kRowsA);
+  if (rc) return rc;
+  rc = encode_operand(&map_b, narrow ? lhs : rhs, rows_b, d.k, narrow ? lhs_row_stride : rhs_row_stride, c.tile);
+  if (rc) return rc;
+  if (p.tma_store) {
+    const uint64_t dims[2] = {static_cast<uint64_t>(d.n), static_cast<uint64_t>(m)};
+    const uint64_t strides[1] = {static_cast<uint64_t>(out_row_stride) * osize};
+    const uint32_t box[2] = {32, 32};
+    rc = cake::encode_tensor_map_as(&map_out, out, 2, dims, strides, box, osize == 4 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                                    osize == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16);
+    if (rc) return rc;
+  }
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  switch (c.tile) {
+    case 16: return launch<16, true>(plan, map_a, map_b, map_out, p, s);
+    case 32: return launch<32, true>(plan, map_a, map_b, map_out, p, s);
+    case 64: return launch<64, true>(plan, map_a, map_b, map_out, p, s);
+    case 128: return launch<128, false>(plan, map_a, map_b, map_out, p, s);
+    case 192: return launch<192, false>(plan, map_a, map_b, map_out, p, s);
+    default: return launch<224, false>(plan, map_a, map_b, map_out, p, s);
+  }
+}
+
+int32_t cake_scaled_matmul_status(cake_scaled_matmul* plan, void* stream, cake_status* out) {
+  if (!plan || !out) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_status: null argument");
+  const int32_t rc = plan->status.read_and_clear(static_cast<cudaStream_t>(stream), out);
+  if (rc) return rc;
+  if (out->code == 1)
+    return fail(CAKE_ERR_TIMEOUT, "device-side bounded wait ran out: block=%d tile=%d where=%d", out->detail0, out->detail1, out->detail2);
+  return CAKE_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,294 @@
+"""CUDA backend plans of the 8-bit linear layer: row quantisation, RMS norm with 8-bit output, and the
+block-scaled matmul that takes both.
+
+The reference has one matmul, in bf16 (src/tpu_cake/pallas_lowering.py:44-50); ``CudaScaledMatmulPlan``
+is its local contraction at half the bytes and twice the tensor rate, and the two row plans make its
+operands. Operands are pairs (codes, scales): codes ``torch.float8_e4m3fn`` [rows, columns] with
+contiguous rows whose pitch is a multiple of 16 bytes, scales ``torch.float8_e8m0fnu``
+[rows, ceil(columns / 128)], one power of two per 128 consecutive columns of a row:
+
+  scale   the least 2^e >= 2^-127 with max |v| <= 448 * 2^e over the group; 1 for a group of zeros; NaN
+          for a group that holds an infinity or a NaN, whose codes are then NaN throughout
+  code    v / scale rounded to nearest even
+
+Plans are built for a width and a type and serve any number of rows, zero included. Calls are
+asynchronous on the device's current stream, allocate their outputs from torch unless they are given,
+use no workspace and keep nothing between calls, so they can be captured into CUDA graphs.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _native
+from .identity import text_sha256
+
+GROUP_COLUMNS = 128
+CODE_DTYPE = torch.float8_e4m3fn
+SCALE_DTYPE = torch.float8_e8m0fnu
+MAX_NORM_COLUMNS = 32768
+_DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+_CAKE_DTYPES = {"bf16": _native.CAKE_DTYPE_BF16, "f16": _native.CAKE_DTYPE_F16, "f32": _native.CAKE_DTYPE_F32}
+_GATES = {"none": _native.CAKE_GATE_NONE, "silu": _native.CAKE_GATE_SILU}
+
+
+def scale_columns(columns: int) -> int:
+    """Scales of a row of ``columns`` codes."""
+    return -(-columns // GROUP_COLUMNS)
+
+
+def empty_codes(rows: int, columns: int, device: torch.device) -> torch.Tensor:
+    """Uninitialised codes with the row pitch the matmul wants (a multiple of 16 bytes)."""
+    pitch = -(-columns // 16) * 16
+    codes = torch.empty((rows, pitch), dtype=CODE_DTYPE, device=device)
+    return codes if pitch == columns else codes[:, :columns]
+
+
+def empty_scales(rows: int, columns: int, device: torch.device) -> torch.Tensor:
+    return torch.empty((rows, scale_columns(columns)), dtype=SCALE_DTYPE, device=device)
+
+
+def _rows(tensor, columns: int, dtype: torch.dtype, name: str, device: torch.device, rows: int | None = None) -> int:
+    """Checks a row operand (contiguous rows, any row stride that does not overlap) and returns its rows."""
+    if not isinstance(tensor, torch.Tensor) or tensor.dtype != dtype or tensor.dim() != 2 or tensor.shape[1] != columns \
+            or (rows is not None and tensor.shape[0] != rows):
+        got = (tuple(tensor.shape), tensor.dtype) if isinstance(tensor, torch.Tensor) else type(tensor)
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {('rows' if rows is None else rows, columns)}, got {got}")
+    if tensor.device != device:
+        raise ValueError(f"{name} must be on {device}, is on {tensor.device}")
+    count = tensor.shape[0]
+    if (columns > 1 and tensor.stride(1) != 1) or (count > 1 and tensor.stride(0) < columns):
+        raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {tensor.stride()}")
+    return count
+
+
+class _Executable:
+    """The library and the device a plan was built on."""
+
+    def __init__(self, device: torch.device):
+        self._lib = _native.load()
+        self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
+
+    def _stream(self) -> int:
+        return torch.cuda.current_stream(self.device).cuda_stream
+
+    def _call(self, entry, *arguments) -> None:
+        """Enqueues on the device's current stream. The library launches on the current device."""
+        if torch.cuda.current_device() == self.device.index:
+            code = entry(*arguments, self._stream())
+        else:
+            with torch.cuda.device(self.device):
+                code = entry(*arguments, self._stream())
+        if code != _native.CAKE_OK:
+            _native.check(code)
+
+    def close(self) -> None:
+        pass
+
+
+class RowQuantizeExecutable(_Executable):
+    """The row kernels keep nothing: a device and the library."""
+
+    def quantize(self, *arguments) -> None:
+        self._call(self._lib.cake_quantize_rows_enqueue, *arguments)
+
+    def rms_norm_quantize(self, *arguments) -> None:
+        self._call(self._lib.cake_rms_norm_quantize_enqueue, *arguments)
+
+
+class ScaledMatmulExecutable(_Executable):
+    """Owns one native plan (its descriptor and a status word) on a GPU."""
+
+    def __init__(self, desc: _native.ScaledMatmulDesc, device: torch.device):
+        super().__init__(device)
+        handle = ctypes.c_void_p()
+        with torch.cuda.device(self.device):
+            _native.check(self._lib.cake_scaled_matmul_create(ctypes.byref(desc), ctypes.byref(handle)))
+        self._handle = handle
+
+    def enqueue(self, *arguments) -> None:
+        if not self._handle:
+            raise RuntimeError("the scaled matmul executable is closed")
+        self._call(self._lib.cake_scaled_matmul_enqueue, self._handle, *arguments)
+
+    def status(self) -> tuple[int, int, int, int]:
+        word = _native.CakeStatus()
+        _native.check(self._lib.cake_scaled_matmul_status(self._handle, self._stream(), ctypes.byref(word)))
+        return (word.code, word.detail0, word.detail1, word.detail2)
+
+    def close(self) -> None:
+        if self._handle:
+            torch.cuda.synchronize(self.device)
+            self._lib.cake_scaled_matmul_destroy(self._handle)
+            self._handle = None
+
+
+def _source(kind: str, kernel: str, plan, fields: tuple[str, ...]) -> str:
+    lines = [f"# cake-b200 lowered {kind}", f"name = {plan.name!r}", f"kernel = {kernel!r}"]
+    lines += [f"{field} = {getattr(plan, field)!r}" for field in fields]
+    return "\n".join([*lines, f"group_columns = {GROUP_COLUMNS}", "codes = 'e4m3'", "scales = 'e8m0'", "abi_version = 1"]) + "\n"
+
+
+def _device(device: torch.device | None) -> torch.device:
+    return device or torch.device("cuda", torch.cuda.current_device())
+
+
+@dataclass(frozen=True)
+class CudaQuantizeRowsPlan:
+    """codes, scales of ``x`` [rows, columns], or with ``gate="silu"`` of silu(gate) * up with ``x`` =
+    [rows, gate | up] (2 * columns wide), computed in f32."""
+
+    name: str
+    columns: int
+    input_dtype: str = "bf16"
+    gate: str = "none"
+
+    def __post_init__(self) -> None:
+        if self.columns < 1:
+            raise ValueError(f"columns must be positive, got {self.columns}")
+        if self.input_dtype not in _DTYPES:
+            raise ValueError(f"input dtype must be one of {tuple(_DTYPES)}, got {self.input_dtype}")
+        if self.gate not in _GATES:
+            raise ValueError(f"gate must be one of {tuple(_GATES)}, got {self.gate}")
+
+    def render_executable_source(self) -> str:
+        return _source("row quantisation", "cake_quantize_rows_sm100", self, ("columns", "input_dtype", "gate"))
+
+    def source_sha256(self) -> str:
+        return text_sha256(self.render_executable_source())
+
+    def build(self, device: torch.device | None = None) -> RowQuantizeExecutable:
+        return RowQuantizeExecutable(_device(device))
+
+    def invoke(self, executable: RowQuantizeExecutable, x, *, codes=None, scales=None) -> tuple[torch.Tensor, torch.Tensor]:
+        device, columns = executable.device, self.columns
+        rows = _rows(x, columns if self.gate == "none" else 2 * columns, _DTYPES[self.input_dtype], "x", device)
+        if codes is None:
+            codes = empty_codes(rows, columns, device)
+        else:
+            _rows(codes, columns, CODE_DTYPE, "codes", device, rows)
+        if scales is None:
+            scales = empty_scales(rows, columns, device)
+        else:
+            _rows(scales, scale_columns(columns), SCALE_DTYPE, "scales", device, rows)
+        executable.quantize(x.data_ptr(), _CAKE_DTYPES[self.input_dtype], x.stride(0), _GATES[self.gate], rows, columns,
+                            codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0))
+        return codes, scales
+
+
+@dataclass(frozen=True)
+class CudaRmsNormQuantizePlan:
+    """codes, scales of h / sqrt(mean(h^2) + epsilon) * weight with h = x + residual (or x alone), all in
+    f32, and h rounded to the input type as the next layer's residual."""
+
+    name: str
+    columns: int
+    input_dtype: str = "bf16"
+    weight_dtype: str = "bf16"
+    epsilon: float = 1e-5
+    with_residual: bool = True
+
+    def __post_init__(self) -> None:
+        if not 1 <= self.columns <= MAX_NORM_COLUMNS:
+            raise ValueError(f"a norm's row is held on chip: columns must be 1 to {MAX_NORM_COLUMNS}, got {self.columns}")
+        if self.input_dtype not in _DTYPES:
+            raise ValueError(f"input dtype must be one of {tuple(_DTYPES)}, got {self.input_dtype}")
+        if self.weight_dtype not in (self.input_dtype, "f32"):
+            raise ValueError(f"weight dtype must be the input's or f32, got {self.weight_dtype}")
+        if not self.epsilon >= 0:
+            raise ValueError(f"epsilon must not be negative, got {self.epsilon}")
+
+    def render_executable_source(self) -> str:
+        return _source("RMS norm with 8-bit output", "cake_rms_norm_quantize_sm100", self,
+                       ("columns", "input_dtype", "weight_dtype", "epsilon", "with_residual"))
+
+    def source_sha256(self) -> str:
+        return text_sha256(self.render_executable_source())
+
+    def build(self, device: torch.device | None = None) -> RowQuantizeExecutable:
+        return RowQuantizeExecutable(_device(device))
+
+    def invoke(self, executable: RowQuantizeExecutable, x, weight, residual=None, *, codes=None, scales=None, residual_out=None):
+        """Returns (codes, scales, new residual or None). ``residual_out`` may be ``residual`` or ``x``."""
+        device, columns, dtype = executable.device, self.columns, _DTYPES[self.input_dtype]
+        rows = _rows(x, columns, dtype, "x", device)
+        if not isinstance(weight, torch.Tensor) or weight.dtype != _DTYPES[self.weight_dtype] or tuple(weight.shape) != (columns,) \
+                or weight.device != device or (columns > 1 and weight.stride(0) != 1):
+            raise ValueError(f"weight must be a contiguous {self.weight_dtype} vector of {columns} on {device}")
+        if (residual is not None) != self.with_residual:
+            raise ValueError("residual must be given to a plan with residual, and to no other")
+        if self.with_residual:
+            _rows(residual, columns, dtype, "residual", device, rows)
+            if residual_out is None:
+                residual_out = torch.empty((rows, columns), dtype=dtype, device=device)
+            else:
+                _rows(residual_out, columns, dtype, "residual_out", device, rows)
+        elif residual_out is not None:
+            raise ValueError("residual_out needs a plan with residual")
+        if codes is None:
+            codes = empty_codes(rows, columns, device)
+        else:
+            _rows(codes, columns, CODE_DTYPE, "codes", device, rows)
+        if scales is None:
+            scales = empty_scales(rows, columns, device)
+        else:
+            _rows(scales, scale_columns(columns), SCALE_DTYPE, "scales", device, rows)
+        executable.rms_norm_quantize(
+            x.data_ptr(), _CAKE_DTYPES[self.input_dtype], x.stride(0),
+            residual.data_ptr() if residual is not None else None, residual.stride(0) if residual is not None else 0,
+            residual_out.data_ptr() if residual is not None else None, residual_out.stride(0) if residual is not None else 0,
+            weight.data_ptr(), _CAKE_DTYPES[self.weight_dtype], self.epsilon, rows, columns,
+            codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0))
+        return codes, scales, residual_out
+
+
+@dataclass(frozen=True)
+class CudaScaledMatmulPlan:
+    """out [m, n] = lhs [m, k] rhs [n, k]^T over dequantised operands, accumulated in f32 and rounded once
+    to ``output_dtype``. ``tile`` and ``k_split`` override the library's choice (0): tiles of 16, 32 or 64
+    tokens by 128 columns with 1 to 8 blocks sharing a tile's contraction, or of 128 tokens by 128,
+    192 or 224 columns. Runs on one mesh position."""
+
+    name: str
+    n: int
+    k: int
+    output_dtype: str = "bf16"
+    tile: int = 0
+    k_split: int = 0
+
+    def __post_init__(self) -> None:
+        if not (0 < self.n < 1 << 30 and 0 < self.k < 1 << 30):
+            raise ValueError(f"scaled matmul extents must be 1 to 2^30 - 1, got n={self.n} k={self.k}")
+        if self.output_dtype not in ("bf16", "f32"):
+            raise ValueError(f"output dtype must be f32 or bf16, got {self.output_dtype}")
+        if self.tile not in (0, 16, 32, 64, 128, 192, 224):
+            raise ValueError(f"tile must be 0, 16, 32, 64, 128, 192 or 224, got {self.tile}")
+        if not 0 <= self.k_split <= 8 or (self.k_split > 1 and self.tile not in (16, 32, 64)):
+            raise ValueError(f"k_split must be 0 to 8, and above 1 only with tile 16, 32 or 64, got {self.k_split}")
+
+    def render_executable_source(self) -> str:
+        return _source("block-scaled matmul", "cake_scaled_matmul_sm100", self, ("n", "k", "output_dtype", "tile", "k_split"))
+
+    def source_sha256(self) -> str:
+        return text_sha256(self.render_executable_source())
+
+    def build(self, device: torch.device | None = None) -> ScaledMatmulExecutable:
+        desc = _native.ScaledMatmulDesc(n=self.n, k=self.k, out_dtype=_CAKE_DTYPES[self.output_dtype], tile=self.tile, k_split=self.k_split, reserved=0)
+        return ScaledMatmulExecutable(desc, _device(device))
+
+    def invoke(self, executable: ScaledMatmulExecutable, lhs, lhs_scales, rhs, rhs_scales, *, out=None) -> torch.Tensor:
+        device, groups, dtype = executable.device, scale_columns(self.k), _DTYPES[self.output_dtype]
+        m = _rows(lhs, self.k, CODE_DTYPE, "lhs", device)
+        _rows(lhs_scales, groups, SCALE_DTYPE, "lhs_scales", device, m)
+        _rows(rhs, self.k, CODE_DTYPE, "rhs", device, self.n)
+        _rows(rhs_scales, groups, SCALE_DTYPE, "rhs_scales", device, self.n)
+        if out is None:
+            out = torch.empty((m, self.n), dtype=dtype, device=device)
+        else:
+            _rows(out, self.n, dtype, "out", device, m)
+        executable.enqueue(m, lhs.data_ptr(), lhs.stride(0), lhs_scales.data_ptr(), lhs_scales.stride(0), rhs.data_ptr(), rhs.stride(0),
+                           rhs_scales.data_ptr(), rhs_scales.stride(0), out.data_ptr(), out.stride(0))
+        return out
