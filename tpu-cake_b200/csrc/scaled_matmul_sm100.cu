@@ -16,7 +16,7 @@
 //           blocks of a cluster, which add their partial sums through distributed shared memory in rank
 //           order (no workspace, no atomics: the same bits every time).
 // Warps: 0 TMA producer (128-byte swizzled rows of 128 codes, one k block per stage), 1 MMA issue and
-// tensor memory, 2 scales, 4-7 epilogue. The scales warp gathers a 32-bit word -- four k blocks' bytes --
+// tensor memory, 2 scales to shared memory, 3 scales on to tensor memory, 4-7 epilogue. Warp 2 gathers a 32-bit word -- four k blocks' bytes --
 // per operand row, so that scales are taken as they lie, with any stride, and puts them into shared memory
 // in the order tcgen05.cp wants: lane i's 16 bytes are rows i, 32 + i, 64 + i, 96 + i.
 #include <cuda_bf16.h>
@@ -34,8 +34,9 @@ constexpr int kThreads = 256;
 constexpr int kRowsA = 128;
 constexpr int kBlockK = 128;  // codes (= bytes) of a k block: one swizzle row, one scale
 constexpr int kUmmaK = 32;
-constexpr int kScaleSlots = 4;          // shared-memory ring of scale words (four k blocks each)
-constexpr int kScaleSets = 2;           // sets of scale columns in tensor memory, used in turn
+constexpr int kScaleSlots = 2;          // shared-memory ring of scales, 16 k blocks (four words a row) each
+constexpr int kSlotWords = 4;
+constexpr int kScaleSets = 3;           // sets of scale columns in tensor memory, used in turn
 constexpr int kStagingSlots = 2;        // 32 x 32 output chunks an epilogue warp may have in flight
 constexpr uint32_t kStagingBytes = 32 * 128;
 constexpr int kReducePitch = kRowsA + 4;  // floats between two tokens' partial sums
@@ -50,9 +51,12 @@ constexpr int pow2_at_least(int v) {
 template <int BN, bool NARROW>
 struct Cfg {
   static constexpr uint32_t kABytes = kRowsA * kBlockK;
-  static constexpr uint32_t kStageBytes = kABytes + BN * kBlockK;
+  static constexpr int kLoadB = NARROW ? BN : BN / 2;  // rows of B that this block loads
+  static constexpr uint32_t kStageBytes = kABytes + kLoadB * kBlockK;
+  static_assert(kStageBytes % 1024 == 0, "swizzle atoms");
   static constexpr int kScaleBlocksB = (BN + 127) / 128;
-  static constexpr uint32_t kScaleSlotBytes = 512 * (1 + kScaleBlocksB);
+  static constexpr uint32_t kWordBytes = 512 * (1 + kScaleBlocksB);  // one word of every operand row
+  static constexpr uint32_t kScaleSlotBytes = kSlotWords * kWordBytes;
   static constexpr uint32_t kStaging = NARROW ? 0 : 4 * kStagingSlots * kStagingBytes;
   // Narrow: two blocks share an SM. Wide: one block has it all.
   static constexpr uint32_t kRoom = (NARROW ? 112 * 1024 : 226 * 1024) - 1024 /*alignment*/ - 512 /*barriers*/;
@@ -102,33 +106,102 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, vol
   }
 }
 
-// Four k blocks' scale bytes of one operand row, from k block kb on; 127 (the number 1) past the row's
-// end and for rows past the operand's, where all codes are zero. ALIGNED: base and stride are multiples
-// of four, and so is kb.
-__device__ __forceinline__ uint32_t scale_word(const uint8_t* scales, int64_t stride, int row, int rows, int kb, int k_blocks, bool aligned) {
-  if (row >= rows) return 0x7F7F7F7Fu;
-  const uint8_t* src = scales + static_cast<int64_t>(row) * stride + kb;
-  if (aligned && kb + 4 <= k_blocks) return __ldg(reinterpret_cast<const uint32_t*>(src));
-  uint32_t w = 0x7F7F7F7Fu;
-  for (int i = 0; i < 4; ++i)
-    if (kb + i < k_blocks) w = (w & ~(0xFFu << (8 * i))) | (static_cast<uint32_t>(src[i]) << (8 * i));
-  return w;
+// The scale bytes of COUNT operand rows for 16 k blocks, from k block kb on, as four words each; 127 (the
+// number 1) past the end. `align`: the rows' addresses and kb are multiples of it (16, 4 or 1). Every branch
+// is the whole warp's and has all rows' loads inside, so that they are under way together: with a branch
+// around each load they ran one after another, and the scales of a word came later than its four k blocks.
+template <int COUNT>
+__device__ __forceinline__ void load_scales(uint32_t (&w)[COUNT][4], const uint8_t* const (&row)[COUNT], int kb, int k_blocks, int align) {
+  if (align == 16 && kb + 16 <= k_blocks) {
+#pragma unroll
+    for (int r = 0; r < COUNT; ++r) {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row[r] + kb));
+      w[r][0] = v.x;
+      w[r][1] = v.y;
+      w[r][2] = v.z;
+      w[r][3] = v.w;
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int at = kb + 4 * i;
+    if (align >= 4 && at + 4 <= k_blocks) {
+#pragma unroll
+      for (int r = 0; r < COUNT; ++r) w[r][i] = __ldg(reinterpret_cast<const uint32_t*>(row[r] + at));
+    } else {
+#pragma unroll
+      for (int r = 0; r < COUNT; ++r) w[r][i] = 0x7F7F7F7Fu;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (at + j < k_blocks) {
+#pragma unroll
+          for (int r = 0; r < COUNT; ++r) w[r][i] ^= (0x7Fu ^ __ldg(row[r] + at + j)) << (8 * j);
+        }
+      }
+    }
+  }
 }
 
-// Consecutive tiles walk 16 row tiles down before moving one column tile right, so that the blocks of a
+__device__ __forceinline__ int scale_alignment(const uint8_t* scales, int64_t stride, int kb_begin) {
+  const uintptr_t bits = reinterpret_cast<uintptr_t>(scales) | static_cast<uintptr_t>(stride) | static_cast<uintptr_t>(kb_begin);
+  return (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;
+}
+
+// Consecutive tiles walk 8 row tiles down before moving one column tile right, so that the blocks of a
 // wave share both operands' rows in L2.
 __device__ __forceinline__ void raster(int t, int tiles_a, int tiles_b, int& ta, int& tb) {
-  const int group = 16 * tiles_b;
+  constexpr int kHigh = 8;
+  const int group = kHigh * tiles_b;
   const int g = t / group;
-  const int rows = min(16, tiles_a - g * 16);
+  const int rows = min(kHigh, tiles_a - g * kHigh);
   const int r = t - g * group;
-  ta = g * 16 + r % rows;
+  ta = g * kHigh + r % rows;
   tb = r / rows;
 }
 
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// The same for a barrier on which the other block of the pair arrives too.
+__device__ __forceinline__ bool wait_or_abort_cluster(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  if (mbar_try_wait_cluster(bar, parity)) return true;
+  const long long start = clock64();
+  while (true) {
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait_cluster(bar, parity)) return true;
+    if (*abort_flag) return false;
+    if (clock64() - start > kBudgetCycles) return false;
+  }
+}
+
+// A whole warp waits: the result is the warp's, so that what follows stays uniform.
+template <bool CLUSTER>
+__device__ __forceinline__ bool wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag) {
+  if (__all_sync(0xffffffffu, CLUSTER ? mbar_try_wait_cluster(bar, parity) : mbar_try_wait(bar, parity))) return true;
+  return __all_sync(0xffffffffu, CLUSTER ? wait_or_abort_cluster(bar, parity, abort_flag) : wait_or_abort(bar, parity, abort_flag));
+}
+
+// One block (narrow) or a pair (wide): the instructions that differ.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+  if (PAIR) tcgen05_commit_pair(bar);
+  else tcgen05_commit(bar);
+}
+
+// The same for a barrier that only the issuing block waits on.
+template <bool PAIR>
+__device__ __forceinline__ void tcgen05_commit_as(uint32_t bar) {
+  if (PAIR) tcgen05_commit_pair_local(bar);
+  else tcgen05_commit(bar);
+}
+
+template <bool PAIR>
+__device__ __forceinline__ void copy_scales(uint32_t dst, uint32_t src) {
+  if (PAIR) tcgen05_cp_32x128b_warpx4_pair(dst, umma_desc_scales(src));
+  else tcgen05_cp_32x128b_warpx4(dst, umma_desc_scales(src));
 }
 
 template <int BN, bool NARROW>
@@ -148,17 +221,22 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
   uint64_t* scale_empty = scale_full + kScaleSlots;
   uint64_t* tmem_full = scale_empty + kScaleSlots;
   uint64_t* tmem_empty = tmem_full + 2;
-  uint64_t* drain_bar = tmem_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 1);
+  uint64_t* set_full = tmem_empty + 2;
+  uint64_t* set_empty = set_full + kScaleSets;
+  uint64_t* drain_bar = set_empty + kScaleSets;  // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain_bar + 2);
   volatile uint32_t* abort_flag = tmem_slot + 1;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int num_tiles = p.tiles_a * p.tiles_b;
-  // Narrow: one tile per cluster, this block's share of its k blocks. Wide: tiles by stride, all k blocks.
-  const int rank = NARROW ? static_cast<int>(blockIdx.x) % p.split : 0;
-  const int first_tile = NARROW ? static_cast<int>(blockIdx.x) / p.split : static_cast<int>(blockIdx.x);
-  const int tile_step = NARROW ? num_tiles : static_cast<int>(gridDim.x);
+  // Narrow: one tile per cluster, this block's share of its k blocks. Wide: tiles by stride, all k blocks;
+  // rank 0 issues for the pair.
+  constexpr bool PAIR = !NARROW;
+  const int rank = static_cast<int>(blockIdx.x) % (NARROW ? p.split : 2);
+  const int first_tile = static_cast<int>(blockIdx.x) / (NARROW ? p.split : 2);
+  const int tile_step = NARROW ? num_tiles : static_cast<int>(gridDim.x) / 2;
+  const bool leader = NARROW || rank == 0;
   const int kb_begin = NARROW ? static_cast<int>(static_cast<int64_t>(p.k_blocks) * rank / p.split) : 0;
   const int kb_end = NARROW ? static_cast<int>(static_cast<int64_t>(p.k_blocks) * (rank + 1) / p.split) : p.k_blocks;
 
@@ -168,25 +246,35 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
       mbar_init(smem_u32(&empty_bar[s]), 1);
     }
     for (int s = 0; s < kScaleSlots; ++s) {
-      mbar_init(smem_u32(&scale_full[s]), 1);
+      mbar_init(smem_u32(&scale_full[s]), PAIR ? 2 : 1);
       mbar_init(smem_u32(&scale_empty[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&tmem_full[b]), 1);
-      mbar_init(smem_u32(&tmem_empty[b]), 4);
+      mbar_init(smem_u32(&tmem_empty[b]), PAIR ? 8 : 4);
     }
-    mbar_init(smem_u32(drain_bar), 1);
+    for (int s = 0; s < kScaleSets; ++s) {
+      mbar_init(smem_u32(&set_full[s]), 1);
+      mbar_init(smem_u32(&set_empty[s]), 1);
+    }
+    mbar_init(smem_u32(&drain_bar[0]), 1);
+    mbar_init(smem_u32(&drain_bar[1]), 1);
     *abort_flag = 0;
     fence_mbar_init();
     prefetch_tensormap(&map_a);
     prefetch_tensormap(&map_b);
   }
   if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
-    tmem_relinquish();
+    if (PAIR) {
+      tmem_alloc_pair(smem_u32(tmem_slot), C::kTmemCols);
+    } else {
+      tmem_alloc(smem_u32(tmem_slot), C::kTmemCols);
+      tmem_relinquish();
+    }
   }
   tcgen05_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // both blocks' barriers exist before either is arrived on
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
   grid_dependency_wait();
@@ -210,9 +298,17 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
           }
           const uint32_t full = smem_u32(&full_bar[stage]);
           const uint32_t dst = smem_u32(smem + stage * C::kStageBytes);
-          mbar_arrive_expect_tx(full, C::kStageBytes);
-          tma_load_2d(dst, &map_a, full, kb * kBlockK, ta * kRowsA);
-          tma_load_2d(dst + C::kABytes, &map_b, full, kb * kBlockK, tb * BN);
+          if (PAIR) {
+            // Both blocks' copies complete on the issuing block's barrier.
+            if (leader) mbar_arrive_expect_tx(full, 2 * C::kStageBytes);
+            const uint32_t bar = cluster_addr(full, 0);
+            tma_load_2d_pair(dst, &map_a, bar, kb * kBlockK, (ta * 2 + rank) * kRowsA);
+            tma_load_2d_pair(dst + C::kABytes, &map_b, bar, kb * kBlockK, tb * BN + rank * C::kLoadB);
+          } else {
+            mbar_arrive_expect_tx(full, C::kStageBytes);
+            tma_load_2d(dst, &map_a, full, kb * kBlockK, ta * kRowsA);
+            tma_load_2d(dst + C::kABytes, &map_b, full, kb * kBlockK, tb * BN);
+          }
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
@@ -220,140 +316,177 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
         }
       }
       if (!ok) {
-        // Let copies in flight land before the block's shared memory is released.
+        // Let copies in flight land before the block's shared memory is released (a pair's both complete
+        // on rank 0's barriers, and rank 1 leaves after rank 0).
         for (int s = 0; s < STAGES; ++s)
           mbar_wait_bounded(smem_u32(&full_bar[s]), s < stage ? phase : (phase ^ 1), 200000000ll);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 && leader) {
     // ------------------------------------------------------------------ MMA issue
-    if (lane == 0) {
-      int stage = 0, it = 0;
-      uint32_t phase = 0;
-      uint32_t words = 0;  // scale words (four k blocks each) brought in so far
-      bool ok = true;
-      for (int t = first_tile; t < num_tiles && ok; t += tile_step, ++it) {
-        const int buf = C::kAccumulators == 2 ? (it & 1) : 0;
-        const uint32_t acc_phase = C::kAccumulators == 2 ? ((it >> 1) & 1) : (it & 1);
-        if (!wait_or_abort(smem_u32(&tmem_empty[buf]), acc_phase ^ 1, abort_flag)) {
-          if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 200 + buf);
+    // The tensor pipe queues next to nothing behind the MMA it works on: what the issuing warp does between
+    // two k blocks shows as soon as it takes longer than one MMA. So this loop is kept to one wait, four
+    // MMAs and one commit per k block (one more of each per four), with the control flow warp-uniform and
+    // the descriptors stepped, not built.
+    const bool issuer = elect_one();
+    const uint64_t desc0 = umma_desc_sw128(smem_u32(smem), 16, 1024);
+    constexpr uint32_t kStageStep = C::kStageBytes >> 4;
+    constexpr uint32_t kIdesc = umma_idesc_mxf8(PAIR ? 2 * kRowsA : kRowsA, BN, 0);
+    uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
+    int it = 0;
+    bool ok = true;
+    for (int t = first_tile; t < num_tiles && ok; t += tile_step, ++it) {
+      const int buf = C::kAccumulators == 2 ? (it & 1) : 0;
+      const uint32_t acc_phase = C::kAccumulators == 2 ? ((it >> 1) & 1) : (it & 1);
+      if (!wait_warp<PAIR>(smem_u32(&tmem_empty[buf]), acc_phase ^ 1, abort_flag)) {
+        if (!*abort_flag && issuer) record(p.status, 1, blockIdx.x, t, 200 + buf);
+        *abort_flag = 1;
+        break;
+      }
+      tcgen05_fence_after();
+      const uint32_t tmem_d = tmem_base + buf * BN;
+      uint32_t accumulate = 0;
+      for (int kb = kb_begin; kb < kb_end && ok; kb += 4) {
+        if (!wait_warp<false>(smem_u32(&set_full[set]), set_phase, abort_flag)) {
+          if (!*abort_flag && issuer) record(p.status, 1, blockIdx.x, t, 500 + set);
           *abort_flag = 1;
+          ok = false;
           break;
         }
-        tcgen05_fence_after();
-        const uint32_t tmem_d = tmem_base + buf * BN;
-        uint32_t sfa = 0;
-        for (int kb = kb_begin; kb < kb_end; ++kb) {
-          const uint32_t byte = static_cast<uint32_t>(kb - kb_begin) & 3u;
-          const uint32_t slot = words % kScaleSlots;
-          if (byte == 0) {
-            // The set of scale columns was last used kScaleSets words ago: the MMAs of that word, whose
-            // completion also freed its slot of the ring, must be done.
-            if (words >= kScaleSets) {
-              const uint32_t old = words - kScaleSets;
-              ok = wait_or_abort(smem_u32(&scale_empty[old % kScaleSlots]), (old / kScaleSlots) & 1, abort_flag);
-            }
-            if (!ok || !wait_or_abort(smem_u32(&scale_full[slot]), (words / kScaleSlots) & 1, abort_flag)) {
-              if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 500 + slot);
-              *abort_flag = 1;
-              ok = false;
-              break;
-            }
-            tcgen05_fence_after();
-            const uint32_t src = smem_u32(scale_ring + slot * C::kScaleSlotBytes);
-            sfa = tmem_base + C::kScaleBase + (words % kScaleSets) * C::kScaleCols;
-            tcgen05_cp_32x128b_warpx4(sfa, umma_desc_scales(src));
+        const uint32_t sfa = tmem_base + C::kScaleBase + set * C::kScaleCols;
 #pragma unroll
-            for (int b = 0; b < C::kScaleBlocksB; ++b)
-              tcgen05_cp_32x128b_warpx4(sfa + 4 + 4 * b, umma_desc_scales(src + 512 * (1 + b)));
-          }
-          if (!wait_or_abort(smem_u32(&full_bar[stage]), phase, abort_flag)) {
-            if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 300 + stage);
+        for (int byte = 0; byte < 4; ++byte) {
+          if (kb + byte >= kb_end) break;
+          if (!wait_warp<false>(smem_u32(&full_bar[stage]), phase, abort_flag)) {
+            if (!*abort_flag && issuer) record(p.status, 1, blockIdx.x, t, 300 + stage);
             *abort_flag = 1;
             ok = false;
             break;
           }
           tcgen05_fence_after();
-          const uint32_t a_addr = smem_u32(smem + stage * C::kStageBytes);
-          const uint32_t b_addr = a_addr + C::kABytes;
-          const uint32_t idesc = umma_idesc_mxf8(kRowsA, BN, 0) | (byte << 4) | (byte << 29);
+          if (issuer) {
+            const uint64_t a_desc = desc0 + stage * kStageStep;
+            const uint64_t b_desc = a_desc + (C::kABytes >> 4);
+            const uint32_t idesc = kIdesc | (byte << 4) | (static_cast<uint32_t>(byte) << 29);
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / kUmmaK; ++kk) {
-            // K-major rows of 128 bytes, groups of eight 1024 bytes apart; a step of 32 codes is 32 bytes
-            // inside the swizzle row.
-            tcgen05_mma_mxf8(tmem_d, umma_desc_sw128(a_addr + kk * kUmmaK, 16, 1024), umma_desc_sw128(b_addr + kk * kUmmaK, 16, 1024),
-                             idesc, sfa, sfa + 4, kb != kb_begin || kk != 0 ? 1u : 0u);
+            for (int kk = 0; kk < kBlockK / kUmmaK; ++kk) {
+              // K-major rows of 128 bytes, groups of eight 1024 bytes apart; a step of 32 codes is 32 bytes
+              // inside the swizzle row.
+              if (PAIR) tcgen05_mma_mxf8_pair(tmem_d, a_desc + kk * (kUmmaK >> 4), b_desc + kk * (kUmmaK >> 4), idesc, sfa, sfa + 4, accumulate);
+              else tcgen05_mma_mxf8(tmem_d, a_desc + kk * (kUmmaK >> 4), b_desc + kk * (kUmmaK >> 4), idesc, sfa, sfa + 4, accumulate);
+              accumulate = 1;
+            }
+            commit<PAIR>(smem_u32(&empty_bar[stage]));
           }
-          tcgen05_commit(smem_u32(&empty_bar[stage]));
-          if (byte == 3 || kb == kb_end - 1) {
-            tcgen05_commit(smem_u32(&scale_empty[slot]));
-            ++words;
-          }
+          accumulate = 1;
           if (++stage == STAGES) {
             stage = 0;
             phase ^= 1;
           }
         }
-        if (ok) tcgen05_commit(smem_u32(&tmem_full[buf]));
+        if (ok && issuer) tcgen05_commit_as<PAIR>(smem_u32(&set_empty[set]));
+        if (++set == kScaleSets) {
+          set = 0;
+          set_phase ^= 1;
+        }
       }
-      // Everything issued above has retired before tensor memory is released.
-      tcgen05_commit(smem_u32(drain_bar));
-      mbar_wait_bounded(smem_u32(drain_bar), 0, kBudgetCycles);
+      if (ok && issuer) commit<PAIR>(smem_u32(&tmem_full[buf]));
+    }
+    // Everything issued above has retired before tensor memory is released.
+    if (issuer) commit<PAIR>(smem_u32(drain_bar));
+    __syncwarp();
+    mbar_wait_bounded(smem_u32(drain_bar), 0, kBudgetCycles);
+  } else if (warp == 3 && leader) {
+    // ------------------------------------------------------------------ scales into tensor memory
+    // Word by word from the ring to one of kScaleSets sets of columns, as soon as the MMAs of the word that
+    // had the set are done; the slot of the ring is free when its last copy is.
+    if (lane == 0) {
+      uint32_t slot = 0, slot_phase = 0, set = 0, set_phase = 0;
+      bool ok = true;
+      for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
+        for (int kb = kb_begin; kb < kb_end; kb += 4) {
+          const int word = ((kb - kb_begin) / 4) % kSlotWords;
+          if (!wait_or_abort(smem_u32(&set_empty[set]), set_phase ^ 1, abort_flag) ||
+              (word == 0 && !wait_or_abort_cluster(smem_u32(&scale_full[slot]), slot_phase, abort_flag))) {
+            if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 700 + slot);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tcgen05_fence_after();
+          const uint32_t src = smem_u32(scale_ring + slot * C::kScaleSlotBytes + word * C::kWordBytes);
+          const uint32_t dst = tmem_base + C::kScaleBase + set * C::kScaleCols;
+#pragma unroll
+          for (int b = 0; b <= C::kScaleBlocksB; ++b) copy_scales<PAIR>(dst + 4 * b, src + 512 * b);
+          tcgen05_commit_as<PAIR>(smem_u32(&set_full[set]));
+          if (word == kSlotWords - 1 || kb + 4 >= kb_end) {
+            commit<PAIR>(smem_u32(&scale_empty[slot]));
+            if (++slot == kScaleSlots) {
+              slot = 0;
+              slot_phase ^= 1;
+            }
+          }
+          if (++set == kScaleSets) {
+            set = 0;
+            set_phase ^= 1;
+          }
+        }
+      }
+      // As above: no copy is under way when tensor memory is released.
+      tcgen05_commit_as<PAIR>(smem_u32(drain_bar + 1));
+      mbar_wait_bounded(smem_u32(drain_bar + 1), 0, kBudgetCycles);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ scales
-    const bool aligned_a = ((reinterpret_cast<uintptr_t>(p.scales_a) | static_cast<uintptr_t>(p.scales_a_stride)) & 3) == 0 && (kb_begin & 3) == 0;
-    const bool aligned_b = ((reinterpret_cast<uintptr_t>(p.scales_b) | static_cast<uintptr_t>(p.scales_b_stride)) & 3) == 0 && (kb_begin & 3) == 0;
-    constexpr int kBlocks = 1 + C::kScaleBlocksB;
-    uint32_t next[kBlocks][4];
-    auto fetch = [&](int ta, int tb, int kb) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        next[0][c] = scale_word(p.scales_a, p.scales_a_stride, ta * kRowsA + c * 32 + lane, p.rows_a, kb, p.k_blocks, aligned_a);
-#pragma unroll
-      for (int b = 1; b < kBlocks; ++b)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int r = (b - 1) * 128 + c * 32;  // of the tile's BN rows; a BN below 32 has lanes past it
-          next[b][c] = r + lane < BN ? scale_word(p.scales_b, p.scales_b_stride, tb * BN + r + lane, p.rows_b, kb, p.k_blocks, aligned_b) : 0x7F7F7F7Fu;
-        }
-    };
-    int slot = 0;
-    uint32_t slot_phase = 0;
-    int t = first_tile, kb = kb_begin, ta = 0, tb = 0;
-    if (t < num_tiles) {
+    // 16 k blocks at a time: the fence and the arrival at cluster scope take some 1500 cycles, which a word
+    // at a time was more than its four k blocks' MMAs. Rows past an operand's end (and past the tile's)
+    // get the last row's scales: their codes are zeros, or not there, and what comes of them is not stored.
+    const int align_a = scale_alignment(p.scales_a, p.scales_a_stride, kb_begin);
+    const int align_b = scale_alignment(p.scales_b, p.scales_b_stride, kb_begin);
+    constexpr int kRowsOfB = (BN + 31) / 32;
+    uint32_t slot = 0, slot_phase = 0;
+    bool ok = true;
+    for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
+      int ta, tb;
       raster(t, p.tiles_a, p.tiles_b, ta, tb);
-      fetch(ta, tb, kb);
-    }
-    while (t < num_tiles) {
-      uint32_t now[kBlocks][4];
+      const uint8_t* row_a[4];
+      const uint8_t* row_b[kRowsOfB];
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
+      for (int c = 0; c < 4; ++c) row_a[c] = p.scales_a + min((PAIR ? ta * 2 + rank : ta) * kRowsA + c * 32 + lane, p.rows_a - 1) * p.scales_a_stride;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) now[b][c] = next[b][c];
-      // The next words are on their way while this slot is waited for.
-      kb += 4;
-      if (kb >= kb_end) {
-        t += tile_step;
-        kb = kb_begin;
-        if (t < num_tiles) raster(t, p.tiles_a, p.tiles_b, ta, tb);
-      }
-      if (t < num_tiles) fetch(ta, tb, kb);
-      if (!__all_sync(0xffffffffu, wait_or_abort(smem_u32(&scale_empty[slot]), slot_phase ^ 1, abort_flag))) {
-        if (!*abort_flag && lane == 0) record(p.status, 1, blockIdx.x, t, 600 + slot);
-        *abort_flag = 1;
-        break;
-      }
+      for (int c = 0; c < kRowsOfB; ++c) row_b[c] = p.scales_b + min(tb * BN + c * 32 + lane, p.rows_b - 1) * p.scales_b_stride;
+      for (int kb = kb_begin; kb < kb_end; kb += 4 * kSlotWords) {
+        uint32_t a[4][4], b[kRowsOfB][4];  // [32 rows each][word]
+        load_scales<4>(a, row_a, kb, p.k_blocks, align_a);
+        load_scales<kRowsOfB>(b, row_b, kb, p.k_blocks, align_b);
+        if (!wait_warp<false>(smem_u32(&scale_empty[slot]), slot_phase ^ 1, abort_flag)) {
+          if (!*abort_flag && lane == 0) record(p.status, 1, blockIdx.x, t, 600 + slot);
+          *abort_flag = 1;
+          ok = false;
+          break;
+        }
+        uint8_t* dst = scale_ring + slot * C::kScaleSlotBytes + lane * 16;
 #pragma unroll
-      for (int b = 0; b < kBlocks; ++b)
-        *reinterpret_cast<uint4*>(scale_ring + slot * C::kScaleSlotBytes + b * 512 + lane * 16) =
-            make_uint4(now[b][0], now[b][1], now[b][2], now[b][3]);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(&scale_full[slot]));
-      if (++slot == kScaleSlots) {
-        slot = 0;
-        slot_phase ^= 1;
+        for (int i = 0; i < kSlotWords; ++i) {
+          *reinterpret_cast<uint4*>(dst + i * C::kWordBytes) = make_uint4(a[0][i], a[1][i], a[2][i], a[3][i]);
+#pragma unroll
+          for (int c = 0; c < kRowsOfB; c += 4) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] = c + j < kRowsOfB ? b[c + j < kRowsOfB ? c + j : 0][i] : 0x7F7F7F7Fu;
+            *reinterpret_cast<uint4*>(dst + i * C::kWordBytes + 512 * (1 + c / 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (PAIR) mbar_arrive_cluster(cluster_addr(smem_u32(&scale_full[slot]), 0));
+          else mbar_arrive(smem_u32(&scale_full[slot]));
+        }
+        if (++slot == kScaleSlots) {
+          slot = 0;
+          slot_phase ^= 1;
+        }
       }
     }
   } else if (warp >= 4) {
@@ -374,7 +507,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
       }
       tcgen05_fence_after();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + buf * BN;
-      const int row0 = ta * kRowsA + q * 32;
+      const int row0 = (PAIR ? ta * 2 + rank : ta) * kRowsA + q * 32;
       if (NARROW) {
         // Lane = output column, register = token. Alone, the block stores 32 columns of a token at a
         // time; sharing the tile, it leaves its partial sums in the operand ring, which is free: the
@@ -416,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
         if (c == BN - 32) {
           tcgen05_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&tmem_empty[buf]));
+          if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&tmem_empty[buf]), 0));
         }
         const int col = tb * BN + c;
         if (row0 >= p.rows_a || col >= p.rows_b) continue;  // warp-uniform
@@ -509,8 +642,12 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
   }
   tcgen05_fence_before();
   __syncthreads();
+  if (PAIR) cluster_sync();  // neither block leaves while the other's instructions may touch it
   tcgen05_fence_after();
-  if (warp == 1) tmem_dealloc(tmem_base, C::kTmemCols);
+  if (warp == 1) {
+    if (PAIR) tmem_dealloc_pair(tmem_base, C::kTmemCols);
+    else tmem_dealloc(tmem_base, C::kTmemCols);
+  }
 }
 
 }  // namespace
@@ -546,16 +683,16 @@ int32_t launch(const cake_scaled_matmul* plan, const CUtensorMap& a, const CUten
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[0].val.programmaticStreamSerializationAllowed = 1;
   attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim.x = NARROW ? p.split : 1;
+  attrs[1].val.clusterDim.x = NARROW ? p.split : 2;
   attrs[1].val.clusterDim.y = 1;
   attrs[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(NARROW ? tiles * p.split : (tiles < plan->sm_count ? tiles : plan->sm_count)));
+  config.gridDim = dim3(static_cast<unsigned>(NARROW ? tiles * p.split : 2 * (tiles < plan->sm_count / 2 ? tiles : plan->sm_count / 2)));
   config.blockDim = dim3(cake::kThreads);
   config.dynamicSmemBytes = C::kSmemBytes;
   config.stream = stream;
   config.attrs = attrs;
-  config.numAttrs = NARROW && p.split > 1 ? 2 : 1;
+  config.numAttrs = NARROW && p.split == 1 ? 1 : 2;
   CAKE_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a, b, out, p));
   return CAKE_OK;
 }
@@ -585,8 +722,9 @@ Choice choose(const cake_scaled_matmul* plan, int64_t m) {
     else {
       int64_t best = 0;
       for (int tile : {128, 192, 224}) {
-        const int64_t tiles = ((m + 127) / 128) * ((d.n + tile - 1) / tile);
-        const int64_t cost = (tiles + plan->sm_count - 1) / plan->sm_count * tile;
+        const int64_t tiles = ((m + 255) / 256) * ((d.n + tile - 1) / tile);
+        const int64_t pairs = plan->sm_count / 2;
+        const int64_t cost = (tiles + pairs - 1) / pairs * tile;
         if (best == 0 || cost <= best) {
           best = cost;
           c.tile = tile;
@@ -687,7 +825,8 @@ int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const vo
   const int64_t rows_a = narrow ? d.n : m, rows_b = narrow ? m : d.n;
   p.rows_a = static_cast<int32_t>(rows_a);
   p.rows_b = static_cast<int32_t>(rows_b);
-  const int64_t tiles_a = (rows_a + cake::kRowsA - 1) / cake::kRowsA, tiles_b = (rows_b + c.tile - 1) / c.tile;
+  const int64_t tile_rows = narrow ? cake::kRowsA : 2 * cake::kRowsA;
+  const int64_t tiles_a = (rows_a + tile_rows - 1) / tile_rows, tiles_b = (rows_b + c.tile - 1) / c.tile;
   if (tiles_a * tiles_b * c.split > INT32_MAX / 2)
     return fail(CAKE_ERR_UNSUPPORTED, "%lld x %lld tiles are more than one launch covers", (long long)tiles_a, (long long)tiles_b);
   p.tiles_a = static_cast<int32_t>(tiles_a);
@@ -711,7 +850,7 @@ int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const vo
   memset(&map_out, 0, sizeof(map_out));
   int32_t rc = encode_operand(&map_a, narrow ? rhs : lhs, rows_a, d.k, narrow ? rhs_row_stride : lhs_row_stride, cake::kRowsA);
   if (rc) return rc;
-  rc = encode_operand(&map_b, narrow ? lhs : rhs, rows_b, d.k, narrow ? lhs_row_stride : rhs_row_stride, c.tile);
+  rc = encode_operand(&map_b, narrow ? lhs : rhs, rows_b, d.k, narrow ? lhs_row_stride : rhs_row_stride, narrow ? c.tile : c.tile / 2);
   if (rc) return rc;
   if (p.tma_store) {
     const uint64_t dims[2] = {static_cast<uint64_t>(d.n), static_cast<uint64_t>(m)};

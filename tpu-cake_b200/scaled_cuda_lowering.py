@@ -42,27 +42,28 @@ def scale_columns(columns: int) -> int:
 
 def empty_codes(rows: int, columns: int, device: torch.device) -> torch.Tensor:
     """Uninitialised codes with the row pitch the matmul wants (a multiple of 16 bytes)."""
-    pitch = -(-columns // 16) * 16
-    codes = torch.empty((rows, pitch), dtype=CODE_DTYPE, device=device)
-    return codes if pitch == columns else codes[:, :columns]
+    if columns % 16 == 0:
+        return torch.empty(rows, columns, dtype=CODE_DTYPE, device=device)
+    return torch.empty(rows, -(-columns // 16) * 16, dtype=CODE_DTYPE, device=device)[:, :columns]
 
 
 def empty_scales(rows: int, columns: int, device: torch.device) -> torch.Tensor:
-    return torch.empty((rows, scale_columns(columns)), dtype=SCALE_DTYPE, device=device)
+    return torch.empty(rows, -(-columns // GROUP_COLUMNS), dtype=SCALE_DTYPE, device=device)
 
 
-def _rows(tensor, columns: int, dtype: torch.dtype, name: str, device: torch.device, rows: int | None = None) -> int:
-    """Checks a row operand (contiguous rows, any row stride that does not overlap) and returns its rows."""
-    if not isinstance(tensor, torch.Tensor) or tensor.dtype != dtype or tensor.dim() != 2 or tensor.shape[1] != columns \
-            or (rows is not None and tensor.shape[0] != rows):
-        got = (tuple(tensor.shape), tensor.dtype) if isinstance(tensor, torch.Tensor) else type(tensor)
-        raise ValueError(f"{name} must be a {dtype} tensor of shape {('rows' if rows is None else rows, columns)}, got {got}")
-    if tensor.device != device:
-        raise ValueError(f"{name} must be on {device}, is on {tensor.device}")
-    count = tensor.shape[0]
-    if (columns > 1 and tensor.stride(1) != 1) or (count > 1 and tensor.stride(0) < columns):
-        raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {tensor.stride()}")
-    return count
+def _rows(tensor, columns: int, dtype: torch.dtype, name: str, device: torch.device, rows: int | None = None) -> tuple[int, int]:
+    """Checks a row operand (contiguous rows, any row stride that does not overlap); returns its rows and
+    row stride. A call's time on the host is its time, for few rows: the good case is one expression."""
+    if isinstance(tensor, torch.Tensor) and tensor.dtype is dtype:
+        shape, strides = tensor.shape, tensor.stride()
+        if len(shape) == 2 and shape[1] == columns and (rows is None or shape[0] == rows):
+            if tensor.device != device:
+                raise ValueError(f"{name} must be on {device}, is on {tensor.device}")
+            if (columns > 1 and strides[1] != 1) or (shape[0] > 1 and strides[0] < columns):
+                raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {strides}")
+            return shape[0], strides[0]
+    got = (tuple(tensor.shape), tensor.dtype) if isinstance(tensor, torch.Tensor) else type(tensor)
+    raise ValueError(f"{name} must be a {dtype} tensor of shape {('rows' if rows is None else rows, columns)}, got {got}")
 
 
 class _Executable:
@@ -71,17 +72,17 @@ class _Executable:
     def __init__(self, device: torch.device):
         self._lib = _native.load()
         self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
-
-    def _stream(self) -> int:
-        return torch.cuda.current_stream(self.device).cuda_stream
+        self._index = self.device.index
 
     def _call(self, entry, *arguments) -> None:
         """Enqueues on the device's current stream. The library launches on the current device."""
-        if torch.cuda.current_device() == self.device.index:
-            code = entry(*arguments, self._stream())
+        # The raw handle: torch.cuda.current_stream builds a Stream object, 3 us of a 15 us call.
+        stream = torch._C._cuda_getCurrentRawStream(self._index)
+        if torch._C._cuda_getDevice() == self._index:
+            code = entry(*arguments, stream)
         else:
             with torch.cuda.device(self.device):
-                code = entry(*arguments, self._stream())
+                code = entry(*arguments, stream)
         if code != _native.CAKE_OK:
             _native.check(code)
 
@@ -116,7 +117,7 @@ class ScaledMatmulExecutable(_Executable):
 
     def status(self) -> tuple[int, int, int, int]:
         word = _native.CakeStatus()
-        _native.check(self._lib.cake_scaled_matmul_status(self._handle, self._stream(), ctypes.byref(word)))
+        _native.check(self._lib.cake_scaled_matmul_status(self._handle, torch._C._cuda_getCurrentRawStream(self._index), ctypes.byref(word)))
         return (word.code, word.detail0, word.detail1, word.detail2)
 
     def close(self) -> None:
@@ -124,6 +125,21 @@ class ScaledMatmulExecutable(_Executable):
             torch.cuda.synchronize(self.device)
             self._lib.cake_scaled_matmul_destroy(self._handle)
             self._handle = None
+
+
+def _outputs(codes, scales, rows: int, columns: int, device: torch.device):
+    """Codes and scales of a row operator with their row strides: the caller's, checked, or new ones."""
+    if codes is None:
+        codes = empty_codes(rows, columns, device)
+        codes_stride = -(-columns // 16) * 16
+    else:
+        _, codes_stride = _rows(codes, columns, CODE_DTYPE, "codes", device, rows)
+    groups = -(-columns // GROUP_COLUMNS)
+    if scales is None:
+        scales, scales_stride = torch.empty(rows, groups, dtype=SCALE_DTYPE, device=device), groups
+    else:
+        _, scales_stride = _rows(scales, groups, SCALE_DTYPE, "scales", device, rows)
+    return codes, scales, codes_stride, scales_stride
 
 
 def _source(kind: str, kernel: str, plan, fields: tuple[str, ...]) -> str:
@@ -165,17 +181,10 @@ class CudaQuantizeRowsPlan:
 
     def invoke(self, executable: RowQuantizeExecutable, x, *, codes=None, scales=None) -> tuple[torch.Tensor, torch.Tensor]:
         device, columns = executable.device, self.columns
-        rows = _rows(x, columns if self.gate == "none" else 2 * columns, _DTYPES[self.input_dtype], "x", device)
-        if codes is None:
-            codes = empty_codes(rows, columns, device)
-        else:
-            _rows(codes, columns, CODE_DTYPE, "codes", device, rows)
-        if scales is None:
-            scales = empty_scales(rows, columns, device)
-        else:
-            _rows(scales, scale_columns(columns), SCALE_DTYPE, "scales", device, rows)
-        executable.quantize(x.data_ptr(), _CAKE_DTYPES[self.input_dtype], x.stride(0), _GATES[self.gate], rows, columns,
-                            codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0))
+        rows, stride = _rows(x, columns if self.gate == "none" else 2 * columns, _DTYPES[self.input_dtype], "x", device)
+        codes, scales, codes_stride, scales_stride = _outputs(codes, scales, rows, columns, device)
+        executable.quantize(x.data_ptr(), _CAKE_DTYPES[self.input_dtype], stride, _GATES[self.gate], rows, columns,
+                            codes.data_ptr(), codes_stride, scales.data_ptr(), scales_stride)
         return codes, scales
 
 
@@ -214,34 +223,26 @@ class CudaRmsNormQuantizePlan:
     def invoke(self, executable: RowQuantizeExecutable, x, weight, residual=None, *, codes=None, scales=None, residual_out=None):
         """Returns (codes, scales, new residual or None). ``residual_out`` may be ``residual`` or ``x``."""
         device, columns, dtype = executable.device, self.columns, _DTYPES[self.input_dtype]
-        rows = _rows(x, columns, dtype, "x", device)
-        if not isinstance(weight, torch.Tensor) or weight.dtype != _DTYPES[self.weight_dtype] or tuple(weight.shape) != (columns,) \
+        rows, stride = _rows(x, columns, dtype, "x", device)
+        if not isinstance(weight, torch.Tensor) or weight.dtype != _DTYPES[self.weight_dtype] or weight.shape != (columns,) \
                 or weight.device != device or (columns > 1 and weight.stride(0) != 1):
             raise ValueError(f"weight must be a contiguous {self.weight_dtype} vector of {columns} on {device}")
         if (residual is not None) != self.with_residual:
             raise ValueError("residual must be given to a plan with residual, and to no other")
-        if self.with_residual:
-            _rows(residual, columns, dtype, "residual", device, rows)
+        residual_ptr, residual_stride, out_ptr, out_stride = None, 0, None, 0
+        if residual is not None:
+            _, residual_stride = _rows(residual, columns, dtype, "residual", device, rows)
             if residual_out is None:
-                residual_out = torch.empty((rows, columns), dtype=dtype, device=device)
+                residual_out, out_stride = torch.empty(rows, columns, dtype=dtype, device=device), columns
             else:
-                _rows(residual_out, columns, dtype, "residual_out", device, rows)
+                _, out_stride = _rows(residual_out, columns, dtype, "residual_out", device, rows)
+            residual_ptr, out_ptr = residual.data_ptr(), residual_out.data_ptr()
         elif residual_out is not None:
             raise ValueError("residual_out needs a plan with residual")
-        if codes is None:
-            codes = empty_codes(rows, columns, device)
-        else:
-            _rows(codes, columns, CODE_DTYPE, "codes", device, rows)
-        if scales is None:
-            scales = empty_scales(rows, columns, device)
-        else:
-            _rows(scales, scale_columns(columns), SCALE_DTYPE, "scales", device, rows)
-        executable.rms_norm_quantize(
-            x.data_ptr(), _CAKE_DTYPES[self.input_dtype], x.stride(0),
-            residual.data_ptr() if residual is not None else None, residual.stride(0) if residual is not None else 0,
-            residual_out.data_ptr() if residual is not None else None, residual_out.stride(0) if residual is not None else 0,
-            weight.data_ptr(), _CAKE_DTYPES[self.weight_dtype], self.epsilon, rows, columns,
-            codes.data_ptr(), codes.stride(0), scales.data_ptr(), scales.stride(0))
+        codes, scales, codes_stride, scales_stride = _outputs(codes, scales, rows, columns, device)
+        executable.rms_norm_quantize(x.data_ptr(), _CAKE_DTYPES[self.input_dtype], stride, residual_ptr, residual_stride, out_ptr, out_stride,
+                                     weight.data_ptr(), _CAKE_DTYPES[self.weight_dtype], self.epsilon, rows, columns,
+                                     codes.data_ptr(), codes_stride, scales.data_ptr(), scales_stride)
         return codes, scales, residual_out
 
 
@@ -281,14 +282,14 @@ class CudaScaledMatmulPlan:
 
     def invoke(self, executable: ScaledMatmulExecutable, lhs, lhs_scales, rhs, rhs_scales, *, out=None) -> torch.Tensor:
         device, groups, dtype = executable.device, scale_columns(self.k), _DTYPES[self.output_dtype]
-        m = _rows(lhs, self.k, CODE_DTYPE, "lhs", device)
-        _rows(lhs_scales, groups, SCALE_DTYPE, "lhs_scales", device, m)
-        _rows(rhs, self.k, CODE_DTYPE, "rhs", device, self.n)
-        _rows(rhs_scales, groups, SCALE_DTYPE, "rhs_scales", device, self.n)
+        m, lhs_stride = _rows(lhs, self.k, CODE_DTYPE, "lhs", device)
+        _, lhs_scales_stride = _rows(lhs_scales, groups, SCALE_DTYPE, "lhs_scales", device, m)
+        _, rhs_stride = _rows(rhs, self.k, CODE_DTYPE, "rhs", device, self.n)
+        _, rhs_scales_stride = _rows(rhs_scales, groups, SCALE_DTYPE, "rhs_scales", device, self.n)
         if out is None:
-            out = torch.empty((m, self.n), dtype=dtype, device=device)
+            out, out_stride = torch.empty(m, self.n, dtype=dtype, device=device), self.n
         else:
-            _rows(out, self.n, dtype, "out", device, m)
-        executable.enqueue(m, lhs.data_ptr(), lhs.stride(0), lhs_scales.data_ptr(), lhs_scales.stride(0), rhs.data_ptr(), rhs.stride(0),
-                           rhs_scales.data_ptr(), rhs_scales.stride(0), out.data_ptr(), out.stride(0))
+            _, out_stride = _rows(out, self.n, dtype, "out", device, m)
+        executable.enqueue(m, lhs.data_ptr(), lhs_stride, lhs_scales.data_ptr(), lhs_scales_stride, rhs.data_ptr(), rhs_stride,
+                           rhs_scales.data_ptr(), rhs_scales_stride, out.data_ptr(), out_stride)
         return out
