@@ -8,11 +8,12 @@
 // largest, which are far below half of e4m3's smallest step: the rounding to e4m3 (nearest even) is the
 // only one after v, whose arithmetic is in 32 bits.
 //
-// Both kernels are bound by HBM: one pass, every byte read and written once, 16 lanes per group with 8
-// elements each (one 16-byte load of a 16-bit type), so a group's maximum is four shuffles.
+// Both kernels are one pass over HBM, every byte read and written once. What stands between them and its rate
+// is instructions, so: a group is 8 lanes of 16 elements (three shuffles for its maximum, and the scale's
+// arithmetic once per 16 elements); the maximum of 16-bit types is taken on their packed bits; f32 arithmetic
+// goes in pairs; whole vectors are loaded and stored without looking at their elements.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 
 #include "cake_host.h"
 #include "cake_ptx.cuh"
@@ -21,128 +22,234 @@ namespace cake {
 namespace {
 
 constexpr int kGroup = 128;  // columns that share a scale
-constexpr int kVec = 8;      // elements of one lane
+constexpr int kVec = 8;      // elements of a vector: one or two 16-byte loads
+constexpr int kGroupLanes = 8;
+constexpr int kLaneVecs = 2;  // vectors of a lane in its group, 64 elements apart: a warp's loads stay contiguous
 constexpr int kQuantThreads = 256;
-constexpr int kQuantUnroll = 4;  // groups in flight per half warp
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+// ------------------------------------------------------------------------------ pairs of f32
 
-template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
-
-// Eight elements as they lie in memory.
-template <typename T>
-struct Raw {
-  static constexpr int kWords = kVec * static_cast<int>(sizeof(T)) / 16;
-  uint4 w[kWords];
+struct F2 {
+  uint64_t v;  // low word first
 };
 
-// Loads elements [0, valid) of the eight at `ptr`; the others are zero. VEC: all loads of whole vectors
-// are 16-byte aligned.
+__device__ __forceinline__ F2 pack2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(F2 a, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.v)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
+// ------------------------------------------------------------------------------ vectors
+
+// Eight elements as they lie in memory: four 32-bit words of a 16-bit type, eight of f32.
+template <typename T>
+struct Raw {
+  static constexpr int kWords = kVec * static_cast<int>(sizeof(T)) / 4;
+  uint32_t w[kWords];
+};
+
+// Loads the vector at `ptr`; elements from `valid` on are zero. VEC: vectors are 16-byte aligned and whole.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_raw(Raw<T>& r, const T* ptr, int valid) {
-  if (VEC && valid >= kVec) {
+  if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < Raw<T>::kWords; ++i) r.w[i] = reinterpret_cast<const uint4*>(ptr)[i];
-    return;
+    for (int i = 0; i < Raw<T>::kWords; i += 4) {
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (valid > 0) v = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(ptr) + i);
+      r.w[i] = v.x;
+      r.w[i + 1] = v.y;
+      r.w[i + 2] = v.z;
+      r.w[i + 3] = v.w;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords; ++i) r.w[i] = 0;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if (i < valid) {
+        if constexpr (sizeof(T) == 4) r.w[i] = reinterpret_cast<const uint32_t*>(ptr)[i];
+        else r.w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(ptr)[i]) << (16 * (i & 1));
+      }
+    }
   }
-  T e[kVec];
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) e[i] = i < valid ? ptr[i] : from_f32<T>(0.f);
-  memcpy(&r, e, sizeof(r));
 }
 
 template <typename T>
-__device__ __forceinline__ void widen(float (&v)[kVec], const Raw<T>& r) {
-  T e[kVec];
-  memcpy(e, &r, sizeof(r));
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) v[i] = to_f32(e[i]);
+__device__ __forceinline__ F2 widen(const Raw<T>& r, int pair);
+template <>
+__device__ __forceinline__ F2 widen<float>(const Raw<float>& r, int pair) {
+  return pack2(__uint_as_float(r.w[2 * pair]), __uint_as_float(r.w[2 * pair + 1]));
+}
+template <>
+__device__ __forceinline__ F2 widen<__nv_bfloat16>(const Raw<__nv_bfloat16>& r, int pair) {
+  return pack2(__uint_as_float(r.w[pair] << 16), __uint_as_float(r.w[pair] & 0xFFFF0000u));
+}
+template <>
+__device__ __forceinline__ F2 widen<__half>(const Raw<__half>& r, int pair) {
+  __half2 h;
+  memcpy(&h, &r.w[pair], 4);
+  const float2 f = __half22float2(h);
+  return pack2(f.x, f.y);
 }
 
-// Stores elements [0, valid) of eight.
-template <typename T, bool VEC>
-__device__ __forceinline__ void store_as(T* ptr, const float (&v)[kVec], int valid) {
-  T e[kVec];
-#pragma unroll
-  for (int i = 0; i < kVec; ++i) e[i] = from_f32<T>(v[i]);
-  if (VEC && valid >= kVec) {
-    Raw<T> r;
-    memcpy(&r, e, sizeof(r));
-#pragma unroll
-    for (int i = 0; i < Raw<T>::kWords; ++i) reinterpret_cast<uint4*>(ptr)[i] = r.w[i];
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < kVec; ++i)
-    if (i < valid) ptr[i] = e[i];
+__device__ __forceinline__ void narrow(uint32_t* w, int pair, F2 v, float) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  w[2 * pair] = __float_as_uint(lo);
+  w[2 * pair + 1] = __float_as_uint(hi);
 }
+__device__ __forceinline__ void narrow(uint32_t* w, int pair, F2 v, __nv_bfloat16) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+  memcpy(&w[pair], &b, 4);
+}
+__device__ __forceinline__ void narrow(uint32_t* w, int pair, F2 v, __half) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  const __half2 h = __floats2half2_rn(lo, hi);
+  memcpy(&w[pair], &h, 4);
+}
+
+// Rounds four pairs to T and stores elements [0, valid).
+template <typename T, bool VEC>
+__device__ __forceinline__ void store_as(T* ptr, const F2* v, int valid) {
+  uint32_t w[Raw<T>::kWords];
+#pragma unroll
+  for (int i = 0; i < kVec / 2; ++i) narrow(w, i, v[i], T());
+  if constexpr (VEC) {
+    if (valid > 0) {
+#pragma unroll
+      for (int i = 0; i < Raw<T>::kWords; i += 4)
+        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(ptr) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) {
+      if (i < valid) {
+        if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(ptr)[i] = w[i];
+        else reinterpret_cast<uint16_t*>(ptr)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------ scale and codes
 
 // Magnitudes are compared as integers: that order is the magnitudes' own, with every NaN above infinity,
-// so a NaN is never lost as it would be by a floating-point maximum.
-__device__ __forceinline__ uint32_t largest_magnitude(const float (&v)[kVec]) {
-  uint32_t a = 0;
+// so a NaN is never lost as it would be by a floating-point maximum. The same holds for the 16-bit types,
+// two at a time.
+__device__ __forceinline__ uint32_t largest(uint32_t a, F2 v) {
+  float lo, hi;
+  unpack2(v, lo, hi);
+  return max(a, max(__float_as_uint(lo) & 0x7FFFFFFFu, __float_as_uint(hi) & 0x7FFFFFFFu));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t largest_raw(uint32_t a, const Raw<T>& r) {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i) a = max(a, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < Raw<T>::kWords; ++i) {
+    if (sizeof(T) == 4) a = max(a, r.w[i] & 0x7FFFFFFFu);
+    else a = __vmaxu2(a, r.w[i] & 0x7FFF7FFFu);
+  }
   return a;
 }
 
-// The maximum over the 16 lanes of a half warp.
-__device__ __forceinline__ uint32_t half_warp_max(uint32_t a) {
+__device__ __forceinline__ uint32_t group_max(uint32_t a) {
 #pragma unroll
-  for (int d = 8; d > 0; d >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, d));
+  for (int d = kGroupLanes / 2; d > 0; d >>= 1) a = max(a, __shfl_xor_sync(0xffffffffu, a, d));
   return a;
+}
+
+// The group's largest magnitude as f32 bits, from the lanes' largest_raw.
+template <typename T>
+__device__ __forceinline__ uint32_t group_max_raw(uint32_t a);
+template <>
+__device__ __forceinline__ uint32_t group_max_raw<float>(uint32_t a) { return group_max(a); }
+__device__ __forceinline__ uint32_t group_max_packed(uint32_t a) {
+#pragma unroll
+  for (int d = kGroupLanes / 2; d > 0; d >>= 1) a = __vmaxu2(a, __shfl_xor_sync(0xffffffffu, a, d));
+  return max(a & 0xFFFFu, a >> 16);
+}
+template <>
+__device__ __forceinline__ uint32_t group_max_raw<__nv_bfloat16>(uint32_t a) { return group_max_packed(a) << 16; }
+template <>
+__device__ __forceinline__ uint32_t group_max_raw<__half>(uint32_t a) {
+  return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(group_max_packed(a)))));
 }
 
 // Scale byte of a group whose largest magnitude has the bits `a`. With a = 1.m * 2^(E - 127) and
-// 448 = 1.75 * 2^8 the exponent is E - 127 - 8, one more where 1.m > 1.75.
+// 448 = 1.75 * 2^8 the exponent is E - 127 - 8, one more where 1.m > 1.75, which is what adding 2 - 1.75 =
+// 0x200000 less one to the bits carries over.
 __device__ __forceinline__ uint32_t scale_byte(uint32_t a) {
-  if (a >= 0x7F800000u) return 255u;
-  if (a == 0) return 127u;
-  const int e = static_cast<int>(a >> 23) - 8 + ((a & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-  return static_cast<uint32_t>(max(e, 0));
+  const int e = max(static_cast<int>((a + 0x1FFFFFu) >> 23) - 8, 0);
+  return a >= 0x7F800000u ? 255u : a == 0 ? 127u : static_cast<uint32_t>(e);
 }
 
-// The eight codes of a lane: v / 2^(byte - 127), rounded to nearest even.
-__device__ __forceinline__ uint2 encode(const float (&v)[kVec], uint32_t byte) {
-  if (byte == 255u) return make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu);
-  const float inv = __uint_as_float((254u - byte) << 23);  // byte <= 247: a normal number
-  uint32_t h[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    h[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i] * inv, v[2 * i + 1] * inv), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(h[0] | (h[1] << 16), h[2] | (h[3] << 16));
+// 2^(127 - byte): a normal number, for bytes up to 247; NaN for byte 255, which makes every code NaN.
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float(byte == 255u ? 0x7FC00000u : (254u - byte) << 23); }
+
+// Four values to codes, rounded to nearest even.
+__device__ __forceinline__ uint32_t to_codes(F2 a, F2 b) {
+  float a0, a1, b0, b1;
+  unpack2(a, a0, a1);
+  unpack2(b, b0, b1);
+  uint32_t r;
+  asm("{\n\t"
+      ".reg .b16 l, h;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\t"
+      "cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+      "mov.b32 %0, {l, h};\n\t"
+      "}"
+      : "=r"(r)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+  return r;
 }
 
-// Stores codes [0, valid) of eight; whole vectors as one 8-byte store where VEC says they are aligned.
+// Stores a vector's codes [0, valid); VEC: as one 8-byte store.
 template <bool VEC>
-__device__ __forceinline__ void store_codes(uint8_t* ptr, uint2 codes, int valid) {
-  if (VEC && valid >= kVec) {
-    *reinterpret_cast<uint2*>(ptr) = codes;
-    return;
-  }
-  const uint64_t all = (static_cast<uint64_t>(codes.y) << 32) | codes.x;
+__device__ __forceinline__ void store_codes(uint8_t* ptr, const F2* v, F2 inverse, int valid) {
+  const uint32_t lo = to_codes(mul2(v[0], inverse), mul2(v[1], inverse)), hi = to_codes(mul2(v[2], inverse), mul2(v[3], inverse));
+  if constexpr (VEC) {
+    if (valid > 0) *reinterpret_cast<uint2*>(ptr) = make_uint2(lo, hi);
+  } else {
 #pragma unroll
-  for (int i = 0; i < kVec; ++i)
-    if (i < valid) ptr[i] = static_cast<uint8_t>(all >> (8 * i));
+    for (int i = 0; i < kVec; ++i)
+      if (i < valid) ptr[i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));
+  }
 }
+
+// Elements of the vector at `col` that a row of `cols` has. VEC: all or none.
+template <bool VEC>
+__device__ __forceinline__ int valid_at(int col, int cols) {
+  if (VEC) return col < cols ? kVec : 0;
+  return min(max(cols - col, 0), kVec);
+}
+
+// ------------------------------------------------------------------------------ quantise
 
 // Division by a number known at launch, for dividends below 2^31: multiply, shift.
 struct FastDivisor {
   uint32_t d, magic, shift;
 };
 
-__device__ __forceinline__ uint32_t divide(uint32_t n, const FastDivisor& f) {
-  return (__umulhi(n, f.magic) + n) >> f.shift;
-}
+__device__ __forceinline__ uint32_t divide(uint32_t n, const FastDivisor& f) { return (__umulhi(n, f.magic) + n) >> f.shift; }
 
 FastDivisor fast_divisor(uint32_t d) {
   FastDivisor f;
@@ -157,60 +264,105 @@ struct QuantizeParams {
   const void* x;
   uint8_t* q;
   uint8_t* scales;
-  int64_t x_stride, q_stride, scales_stride;  // elements (bytes) between rows
-  int64_t items;                              // rows * groups
+  int64_t items;                               // rows * groups
+  uint32_t x_stride, q_stride, scales_stride;  // elements (bytes) between rows
   int32_t cols, groups;
   FastDivisor by_groups;
 };
 
-// x / (1 + exp(-x)). For x below about -88 the exponential is infinite and the result -0.
-__device__ __forceinline__ float silu(float x) { return x / (1.f + expf(-x)); }
+// silu(x) = x / (1 + exp(-x)), from z = exp(-|x|) <= 1: x (x < 0 ? z : 1) / (1 + z), which neither overflows
+// nor cancels. z = 2^(hi + lo), hi the rounded and lo the lost part of -|x| log2(e), so that far from zero the
+// exponent's rounding does not show; 1 / (1 + z) by one Newton-Raphson step on the hardware's estimate.
+// Relative error below 10 * 2^-24: the estimate of 2^hi 4, its correction 1, the sum 1, its reciprocal 2, the
+// products 2.
+__device__ __forceinline__ float silu(float x) {
+  constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596303e-8f;  // their sum is log2(e) to 2^-49
+  constexpr float kLn2 = 0.693147182f;
+  const float a = fminf(fabsf(x), 128.f);  // exp(-128) is zero in f32; a NaN comes back with the factor x
+  const float hi = -a * kLog2e;
+  const float lo = fmaf(-a, kLog2eRest, fmaf(-a, kLog2e, -hi));
+  float z, y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(z) : "f"(hi));
+  z = fmaf(z, lo * kLn2, z);
+  const float d = 1.f + z;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(d));
+  y = fmaf(y, fmaf(-d, y, 1.f), y);
+  return x * (x < 0.f ? z : 1.f) * y;
+}
 
-// A half warp takes kQuantUnroll groups that are 16 apart, so that a block's groups lie next to each
-// other and every lane has that many loads in flight.
+// A lane takes UNROLL groups that are 32 apart, so that a block's groups lie next to each other and every
+// lane has that many groups' loads in flight.
 template <typename T, bool GATE, bool VEC>
 __global__ void __launch_bounds__(kQuantThreads) cake_quantize_rows_sm100(const __grid_constant__ QuantizeParams p) {
+  constexpr int kUnroll = (sizeof(T) == 4 || GATE) ? 2 : 4;
+  constexpr int kApart = kQuantThreads / kGroupLanes;
   grid_dependency_wait();
   grid_dependency_trigger();
-  const int lane = threadIdx.x & 15;
-  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kQuantUnroll * (kQuantThreads / 16)) + (threadIdx.x >> 4);
-  int64_t row[kQuantUnroll];
-  int group[kQuantUnroll], valid[kQuantUnroll];
-  Raw<T> x[kQuantUnroll], up[GATE ? kQuantUnroll : 1];
+  const int lane = threadIdx.x % kGroupLanes;
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * (kUnroll * kApart) + threadIdx.x / kGroupLanes;
+  uint32_t row[kUnroll];
+  int col[kUnroll];
+  bool live[kUnroll];
+  Raw<T> x[kUnroll][kLaneVecs], up[GATE ? kUnroll : 1][kLaneVecs];
 #pragma unroll
-  for (int u = 0; u < kQuantUnroll; ++u) {
-    const int64_t item = first + u * (kQuantThreads / 16);
+  for (int u = 0; u < kUnroll; ++u) {
+    const int64_t item = first + u * kApart;
+    live[u] = item < p.items;
+    uint32_t group;
     if (p.items < (1ll << 31)) {
-      const uint32_t r = divide(static_cast<uint32_t>(item), p.by_groups);  // item < items + 64: also below 2^31 + 64
-      row[u] = r;
-      group[u] = static_cast<int>(static_cast<uint32_t>(item) - r * p.by_groups.d);
+      row[u] = divide(static_cast<uint32_t>(item), p.by_groups);
+      group = static_cast<uint32_t>(item) - row[u] * p.by_groups.d;
     } else {
-      row[u] = item / p.groups;
-      group[u] = static_cast<int>(item - row[u] * p.groups);
+      row[u] = static_cast<uint32_t>(item / p.groups);
+      group = static_cast<uint32_t>(item - static_cast<int64_t>(row[u]) * p.groups);
     }
-    // Items past the end have nothing valid: they load and store nothing.
-    valid[u] = item < p.items ? min(max(p.cols - (group[u] * kGroup + lane * kVec), 0), kVec) : 0;
-    const T* src = static_cast<const T*>(p.x) + row[u] * p.x_stride + group[u] * kGroup + lane * kVec;
-    load_raw<T, VEC>(x[u], src, valid[u]);
-    if (GATE) load_raw<T, VEC>(up[GATE ? u : 0], src + p.cols, valid[u]);
+    col[u] = static_cast<int>(group) * kGroup + lane * kVec;
+    const T* src = static_cast<const T*>(p.x) + static_cast<uint64_t>(row[u]) * p.x_stride + col[u];
+#pragma unroll
+    for (int v = 0; v < kLaneVecs; ++v) {
+      // Items past the end load and store nothing.
+      const int valid = live[u] ? valid_at<VEC>(col[u] + v * kGroupLanes * kVec, p.cols) : 0;
+      load_raw<T, VEC>(x[u][v], src + v * kGroupLanes * kVec, valid);
+      if (GATE) load_raw<T, VEC>(up[GATE ? u : 0][v], src + p.cols + v * kGroupLanes * kVec, valid);
+    }
   }
 #pragma unroll
-  for (int u = 0; u < kQuantUnroll; ++u) {
-    float v[kVec];
-    widen<T>(v, x[u]);
+  for (int u = 0; u < kUnroll; ++u) {
+    F2 v[kLaneVecs][kVec / 2];
+    uint32_t a = 0;
     if (GATE) {
-      float w[kVec];
-      widen<T>(w, up[GATE ? u : 0]);
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) v[i] = silu(v[i]) * w[i];
+      for (int k = 0; k < kLaneVecs; ++k)
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) {
+          float lo, hi;
+          unpack2(widen<T>(x[u][k], i), lo, hi);
+          v[k][i] = mul2(pack2(silu(lo), silu(hi)), widen<T>(up[GATE ? u : 0][k], i));
+          a = largest(a, v[k][i]);
+        }
+      a = group_max(a);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kLaneVecs; ++k) a = largest_raw<T>(a, x[u][k]);
+      a = group_max_raw<T>(a);
+#pragma unroll
+      for (int k = 0; k < kLaneVecs; ++k)
+#pragma unroll
+        for (int i = 0; i < kVec / 2; ++i) v[k][i] = widen<T>(x[u][k], i);
     }
-    const uint32_t byte = scale_byte(half_warp_max(largest_magnitude(v)));
-    if (valid[u] > 0) {
-      store_codes<VEC>(p.q + row[u] * p.q_stride + group[u] * kGroup + lane * kVec, encode(v, byte), valid[u]);
-      if (lane == 0) p.scales[row[u] * p.scales_stride + group[u]] = static_cast<uint8_t>(byte);
+    const uint32_t byte = scale_byte(a);
+    const float inverse = inverse_scale(byte);
+    uint8_t* dst = p.q + static_cast<uint64_t>(row[u]) * p.q_stride + col[u];
+#pragma unroll
+    for (int k = 0; k < kLaneVecs; ++k) {
+      const int at = k * kGroupLanes * kVec;
+      store_codes<VEC>(dst + at, v[k], pack2(inverse, inverse), live[u] ? valid_at<VEC>(col[u] + at, p.cols) : 0);
     }
+    if (lane == 0 && live[u]) p.scales[static_cast<uint64_t>(row[u]) * p.scales_stride + col[u] / kGroup] = static_cast<uint8_t>(byte);
   }
 }
+
+// ------------------------------------------------------------------------------ norm
 
 struct NormParams {
   const void* x;
@@ -219,17 +371,17 @@ struct NormParams {
   const void* weight;
   uint8_t* q;
   uint8_t* scales;
-  int64_t x_stride, residual_stride, residual_out_stride, q_stride, scales_stride;
-  int64_t rows;
+  uint32_t x_stride, residual_stride, residual_out_stride, q_stride, scales_stride;
+  uint32_t rows;
   int32_t cols;
   float epsilon;
 };
 
-// THREADS threads hold one row in registers (VECS vectors of eight each, vector i of thread t being
-// number i * THREADS + t of the row), so the sum x + residual is normalised as it is in 32 bits while its
-// rounding is stored, and the stored sum may lie over x or over the residual. Blocks of 32 threads a row
-// carry eight rows.
-template <typename T, typename W, int THREADS, int VECS, bool VEC>
+// THREADS threads hold one row in registers, UNITS units of 16 elements each (unit i * THREADS + t of the row:
+// eight units are a group), so the sum x + residual is normalised as it is in 32 bits while its rounding is
+// stored, and the stored sum may lie over x or over the residual. Blocks have at least 256 threads, for
+// narrow rows several rows.
+template <typename T, typename W, int THREADS, int UNITS, bool VEC>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_quantize_sm100(const __grid_constant__ NormParams p) {
   constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;  // rows of a block
   constexpr int kWarps = THREADS / 32;                      // warps of a row
@@ -238,61 +390,81 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
   grid_dependency_trigger();
   const int t = threadIdx.x % THREADS;
   const int r = threadIdx.x / THREADS;
-  const int64_t row = static_cast<int64_t>(blockIdx.x) * kRows + r;
+  const uint32_t row = blockIdx.x * kRows + r;
   const bool live = row < p.rows;
-  float h[VECS][kVec];
-  Raw<W> weight[VECS];
-  int valid[VECS];
+  // Column of unit i's first vector; the second is 64 further on.
+  auto col_of = [&](int i) { return ((i * THREADS + t) / kGroupLanes) * kGroup + (t % kGroupLanes) * kVec; };
+  F2 h[UNITS][kLaneVecs][kVec / 2];
   {
-    Raw<T> x[VECS], add[VECS];
+    Raw<T> x[UNITS][kLaneVecs], add[UNITS][kLaneVecs];
+    const T* src = static_cast<const T*>(p.x) + static_cast<uint64_t>(row) * p.x_stride;
+    const T* src_add = static_cast<const T*>(p.residual) + static_cast<uint64_t>(row) * p.residual_stride;
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      const int col = (i * THREADS + t) * kVec;
-      valid[i] = live ? min(max(p.cols - col, 0), kVec) : 0;
-      load_raw<T, VEC>(x[i], static_cast<const T*>(p.x) + row * p.x_stride + col, valid[i]);
-      if (p.residual) load_raw<T, VEC>(add[i], static_cast<const T*>(p.residual) + row * p.residual_stride + col, valid[i]);
-    }
+    for (int i = 0; i < UNITS; ++i)
 #pragma unroll
-    for (int i = 0; i < VECS; ++i) load_raw<W, VEC>(weight[i], static_cast<const W*>(p.weight) + (i * THREADS + t) * kVec, valid[i]);
-#pragma unroll
-    for (int i = 0; i < VECS; ++i) {
-      widen<T>(h[i], x[i]);
-      if (p.residual) {
-        float a[kVec];
-        widen<T>(a, add[i]);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) h[i][e] += a[e];
-        store_as<T, VEC>(static_cast<T*>(p.residual_out) + row * p.residual_out_stride + (i * THREADS + t) * kVec, h[i], valid[i]);
+      for (int k = 0; k < kLaneVecs; ++k) {
+        const int col = col_of(i) + k * kGroupLanes * kVec;
+        const int valid = live ? valid_at<VEC>(col, p.cols) : 0;
+        load_raw<T, VEC>(x[i][k], src + col, valid);
+        if (p.residual) load_raw<T, VEC>(add[i][k], src_add + col, valid);
       }
-    }
+    T* dst = static_cast<T*>(p.residual_out) + static_cast<uint64_t>(row) * p.residual_out_stride;
+#pragma unroll
+    for (int i = 0; i < UNITS; ++i)
+#pragma unroll
+      for (int k = 0; k < kLaneVecs; ++k) {
+        const int col = col_of(i) + k * kGroupLanes * kVec;
+#pragma unroll
+        for (int e = 0; e < kVec / 2; ++e) {
+          h[i][k][e] = widen<T>(x[i][k], e);
+          if (p.residual) h[i][k][e] = add2(h[i][k][e], widen<T>(add[i][k], e));
+        }
+        if (p.residual) store_as<T, VEC>(dst + col, h[i][k], live ? valid_at<VEC>(col, p.cols) : 0);
+      }
   }
-  float sum = 0.f;
+  F2 squares = pack2(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < VECS; ++i)
+  for (int i = 0; i < UNITS; ++i)
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) sum = fmaf(h[i][e], h[i][e], sum);
+    for (int k = 0; k < kLaneVecs; ++k)
+#pragma unroll
+      for (int e = 0; e < kVec / 2; ++e) squares = fma2(h[i][k][e], h[i][k][e], squares);
+  float even, odd;
+  unpack2(squares, even, odd);
+  float sum = even + odd;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (kWarps > 1) {
     if ((t & 31) == 0) partial[r][t / 32] = sum;
     __syncthreads();
-    sum = 0.f;
+    sum = (t & 31) < kWarps ? partial[r][t & 31] : 0.f;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) sum += partial[r][w];
+    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   }
   const float scale = 1.f / sqrtf(sum / static_cast<float>(p.cols) + p.epsilon);
 #pragma unroll
-  for (int i = 0; i < VECS; ++i) {
-    float w[kVec];
-    widen<W>(w, weight[i]);
+  for (int i = 0; i < UNITS; ++i) {
+    uint32_t a = 0;
 #pragma unroll
-    for (int e = 0; e < kVec; ++e) h[i][e] = h[i][e] * scale * w[e];
-    const uint32_t byte = scale_byte(half_warp_max(largest_magnitude(h[i])));
-    if (valid[i] > 0) {
-      const int vec = i * THREADS + t;
-      store_codes<VEC>(p.q + row * p.q_stride + vec * kVec, encode(h[i], byte), valid[i]);
-      if ((t & 15) == 0) p.scales[row * p.scales_stride + vec / 16] = static_cast<uint8_t>(byte);
+    for (int k = 0; k < kLaneVecs; ++k) {
+      const int col = col_of(i) + k * kGroupLanes * kVec;
+      Raw<W> weight;  // from L1 or L2: every row of the SM reads them
+      load_raw<W, VEC>(weight, static_cast<const W*>(p.weight) + col, valid_at<VEC>(col, p.cols));
+#pragma unroll
+      for (int e = 0; e < kVec / 2; ++e) {
+        h[i][k][e] = mul2(mul2(h[i][k][e], pack2(scale, scale)), widen<W>(weight, e));
+        a = largest(a, h[i][k][e]);
+      }
     }
+    const uint32_t byte = scale_byte(group_max(a));
+    const float inverse = inverse_scale(byte);
+#pragma unroll
+    for (int k = 0; k < kLaneVecs; ++k) {
+      const int col = col_of(i) + k * kGroupLanes * kVec;
+      store_codes<VEC>(p.q + static_cast<uint64_t>(row) * p.q_stride + col, h[i][k], pack2(inverse, inverse), live ? valid_at<VEC>(col, p.cols) : 0);
+    }
+    const int col = col_of(i);
+    if (t % kGroupLanes == 0 && live && col < p.cols) p.scales[static_cast<uint64_t>(row) * p.scales_stride + col / kGroup] = static_cast<uint8_t>(byte);
   }
 }
 
@@ -329,12 +501,14 @@ int32_t check_output(const char* who, const void* x, int32_t dtype, int64_t rows
   if (!aligned(x, dtype_size(dtype))) return fail(CAKE_ERR_INVALID_ARGUMENT, "%s: x is not aligned to its elements", who);
   if (rows > 1 && (x_stride < x_cols || q_stride < cols || scales_stride < (cols + kGroup - 1) / kGroup))
     return fail(CAKE_ERR_INVALID_ARGUMENT, "%s: a row stride is shorter than its row", who);
+  if (rows > 1 && (x_stride > UINT32_MAX || q_stride > UINT32_MAX || scales_stride > UINT32_MAX))
+    return fail(CAKE_ERR_UNSUPPORTED, "%s: row strides must be below 2^32", who);
   return CAKE_OK;
 }
 
 template <typename T>
 int32_t launch_quantize(const QuantizeParams& p, bool gate, bool vec, void* stream) {
-  const int64_t per_block = kQuantUnroll * (kQuantThreads / 16);
+  const int64_t per_block = ((sizeof(T) == 4 || gate) ? 2 : 4) * (kQuantThreads / kGroupLanes);
   const unsigned grid = static_cast<unsigned>((p.items + per_block - 1) / per_block);
   void (*kernel)(QuantizeParams) = gate ? (vec ? cake_quantize_rows_sm100<T, true, true> : cake_quantize_rows_sm100<T, true, false>)
                                         : (vec ? cake_quantize_rows_sm100<T, false, true> : cake_quantize_rows_sm100<T, false, false>);
@@ -343,12 +517,13 @@ int32_t launch_quantize(const QuantizeParams& p, bool gate, bool vec, void* stre
 
 template <typename T, typename W, bool VEC>
 int32_t launch_norm_vec(const NormParams& p, void* stream) {
-  const int64_t vectors = (p.cols + kVec - 1) / kVec;
-  if (vectors <= 32 * 4) return launch(cake_rms_norm_quantize_sm100<T, W, 32, 4, VEC>, p, static_cast<unsigned>((p.rows + 7) / 8), 256, stream);
-  if (vectors <= 128 * 4) return launch(cake_rms_norm_quantize_sm100<T, W, 128, 4, VEC>, p, static_cast<unsigned>((p.rows + 1) / 2), 256, stream);
-  if (vectors <= 256 * 4) return launch(cake_rms_norm_quantize_sm100<T, W, 256, 4, VEC>, p, static_cast<unsigned>(p.rows), 256, stream);
-  if (vectors <= 512 * 4) return launch(cake_rms_norm_quantize_sm100<T, W, 512, 4, VEC>, p, static_cast<unsigned>(p.rows), 512, stream);
-  return launch(cake_rms_norm_quantize_sm100<T, W, 1024, 4, VEC>, p, static_cast<unsigned>(p.rows), 1024, stream);
+  const int units = (p.cols + kGroup - 1) / kGroup * kGroupLanes;
+  if (units <= 32) return launch(cake_rms_norm_quantize_sm100<T, W, 32, 1, VEC>, p, (p.rows + 7) / 8, 256, stream);
+  if (units <= 64) return launch(cake_rms_norm_quantize_sm100<T, W, 32, 2, VEC>, p, (p.rows + 7) / 8, 256, stream);
+  if (units <= 256) return launch(cake_rms_norm_quantize_sm100<T, W, 128, 2, VEC>, p, (p.rows + 1) / 2, 256, stream);
+  if (units <= 512) return launch(cake_rms_norm_quantize_sm100<T, W, 256, 2, VEC>, p, p.rows, 256, stream);
+  if (units <= 1024) return launch(cake_rms_norm_quantize_sm100<T, W, 512, 2, VEC>, p, p.rows, 512, stream);
+  return launch(cake_rms_norm_quantize_sm100<T, W, 1024, 2, VEC>, p, p.rows, 1024, stream);
 }
 
 template <typename T>
@@ -376,16 +551,16 @@ int32_t cake_quantize_rows_enqueue(const void* x, int32_t dtype, int64_t x_row_s
   p.x = x;
   p.q = static_cast<uint8_t*>(q);
   p.scales = static_cast<uint8_t*>(scales);
-  p.x_stride = x_row_stride;
-  p.q_stride = q_row_stride;
-  p.scales_stride = scales_row_stride;
+  p.x_stride = static_cast<uint32_t>(rows > 1 ? x_row_stride : 0);
+  p.q_stride = static_cast<uint32_t>(rows > 1 ? q_row_stride : 0);
+  p.scales_stride = static_cast<uint32_t>(rows > 1 ? scales_row_stride : 0);
   p.cols = static_cast<int32_t>(cols);
   p.groups = static_cast<int32_t>((cols + kGroup - 1) / kGroup);
   p.items = rows * p.groups;
   p.by_groups = fast_divisor(static_cast<uint32_t>(p.groups));
-  if (p.items > static_cast<int64_t>(INT32_MAX) * 64) return fail(CAKE_ERR_UNSUPPORTED, "%s: %lld groups are more than one launch covers", who, (long long)p.items);
+  if (p.items > static_cast<int64_t>(INT32_MAX) * 32) return fail(CAKE_ERR_UNSUPPORTED, "%s: %lld groups are more than one launch covers", who, (long long)p.items);
   const int size = dtype_size(dtype);
-  const bool vec = aligned(x, 16) && (rows == 1 || (x_row_stride * size % 16 == 0 && q_row_stride % 8 == 0)) &&
+  const bool vec = cols % kVec == 0 && aligned(x, 16) && (rows == 1 || (x_row_stride * size % 16 == 0 && q_row_stride % 8 == 0)) &&
                    (!gate || cols * size % 16 == 0) && aligned(q, 8);
   if (dtype == CAKE_DTYPE_F32) return launch_quantize<float>(p, gate != 0, vec, stream);
   if (dtype == CAKE_DTYPE_BF16) return launch_quantize<__nv_bfloat16>(p, gate != 0, vec, stream);
@@ -412,6 +587,8 @@ int32_t cake_rms_norm_quantize_enqueue(const void* x, int32_t dtype, int64_t x_r
     return fail(CAKE_ERR_INVALID_ARGUMENT, "%s: an operand is not aligned to its elements", who);
   if (residual && rows > 1 && (residual_row_stride < cols || residual_out_row_stride < cols))
     return fail(CAKE_ERR_INVALID_ARGUMENT, "%s: a row stride is shorter than its row", who);
+  if (residual && rows > 1 && (residual_row_stride > UINT32_MAX || residual_out_row_stride > UINT32_MAX))
+    return fail(CAKE_ERR_UNSUPPORTED, "%s: row strides must be below 2^32", who);
   NormParams p;
   p.x = x;
   p.residual = residual;
@@ -419,17 +596,17 @@ int32_t cake_rms_norm_quantize_enqueue(const void* x, int32_t dtype, int64_t x_r
   p.weight = weight;
   p.q = static_cast<uint8_t*>(q);
   p.scales = static_cast<uint8_t*>(scales);
-  p.x_stride = x_row_stride;
-  p.residual_stride = residual_row_stride;
-  p.residual_out_stride = residual_out_row_stride;
-  p.q_stride = q_row_stride;
-  p.scales_stride = scales_row_stride;
-  p.rows = rows;
+  p.x_stride = static_cast<uint32_t>(rows > 1 ? x_row_stride : 0);
+  p.residual_stride = static_cast<uint32_t>(rows > 1 ? residual_row_stride : 0);
+  p.residual_out_stride = static_cast<uint32_t>(rows > 1 ? residual_out_row_stride : 0);
+  p.q_stride = static_cast<uint32_t>(rows > 1 ? q_row_stride : 0);
+  p.scales_stride = static_cast<uint32_t>(rows > 1 ? scales_row_stride : 0);
+  p.rows = static_cast<uint32_t>(rows);
   p.cols = static_cast<int32_t>(cols);
   p.epsilon = epsilon;
   const bool strides = rows == 1 || (x_row_stride * size % 16 == 0 && q_row_stride % 8 == 0 &&
                                      (!residual || (residual_row_stride * size % 16 == 0 && residual_out_row_stride * size % 16 == 0)));
-  const bool vec = strides && aligned(x, 16) && aligned(residual, 16) && aligned(residual_out, 16) && aligned(weight, 16) && aligned(q, 8);
+  const bool vec = cols % kVec == 0 && strides && aligned(x, 16) && aligned(residual, 16) && aligned(residual_out, 16) && aligned(weight, 16) && aligned(q, 8);
   if (dtype == CAKE_DTYPE_F32) return launch_norm<float>(p, true, vec, stream);
   if (dtype == CAKE_DTYPE_BF16) return launch_norm<__nv_bfloat16>(p, weight_dtype == dtype, vec, stream);
   return launch_norm<__half>(p, weight_dtype == dtype, vec, stream);
