@@ -299,7 +299,8 @@ int32_t cake_rpa_launches_per_enqueue(const cake_rpa* plan);
  * x to its elements is taken; 16-byte aligned rows are faster. */
 
 #define CAKE_GATE_NONE 0
-#define CAKE_GATE_SILU 1 /* x is [rows, 2 cols]: gate | up; v = gate / (1 + exp(-gate)) * up */
+#define CAKE_GATE_SILU 1 /* x is [rows, 2 cols]: gate | up; v = gate / (1 + exp(-gate)) * up in f32, -0 * up
+                            for gates below -87.3, where exp(-gate) passes 2^126 */
 
 /* x: dtype [rows, cols] -> q, scales. Nothing but the groups' own codes and scales is written. */
 int32_t cake_quantize_rows_enqueue(const void* x, int32_t dtype, int64_t x_row_stride, int32_t gate,

@@ -3,9 +3,9 @@
 Tolerances. Quantising x itself is exact: codes and scales equal the oracle's. After arithmetic in f32 (gate,
 norm) a value v may differ from the oracle's by a relative DELTA before it is rounded, so the code times its
 scale lies within half a step of the exact v moved by that much: 2^-4 |v| for normal codes (three mantissa
-bits), 2^-10 s below 2^-6. DELTA for silu(g) u: 2^t within 2^-22 (the hardware estimate's documented bound) and its
-correction, a sum, a reciprocal after one Newton step and three products: 4 + 1 + 1 + 2 + 3 = 11 times 2^-24, below
-2^-20. For the norm: at most 40 sequential and 15 tree additions of squares (half of
+bits), 2^-10 s below 2^-6. DELTA for silu(g) u: 2^t within 2^-22 and the reciprocal within 2^-23 (the
+hardware estimates' documented bounds), a correction, a sum and two products: 4 + 2 + 1 + 1 + 2 = 10 times 2^-24,
+below 2^-20. For the norm: at most 40 sequential and 15 tree additions of squares (half of
 that error reaches the root), quotient, root, two products: below 64 * 2^-24 = 2^-18.
 Matmul: products of codes and powers of two are exact in f32; k additions in f32 are off by at most
 k 2^-24 S with S = sum |lhs| |rhs|, and the output's own rounding by 2^-8 |out| (bf16) or nothing (f32).

@@ -155,10 +155,12 @@ __device__ __forceinline__ void store_as(T* ptr, const F2* v, int valid) {
 // Magnitudes are compared as integers: that order is the magnitudes' own, with every NaN above infinity,
 // so a NaN is never lost as it would be by a floating-point maximum. The same holds for the 16-bit types,
 // two at a time.
-__device__ __forceinline__ uint32_t largest(uint32_t a, F2 v) {
-  float lo, hi;
+// (f32 values in registers go through the hardware's NaN-keeping maximum of magnitudes, three at a time.)
+__device__ __forceinline__ float largest_abs(float a, F2 v) {
+  float lo, hi, r;
   unpack2(v, lo, hi);
-  return max(a, max(__float_as_uint(lo) & 0x7FFFFFFFu, __float_as_uint(hi) & 0x7FFFFFFFu));
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(lo), "f"(hi));
+  return r;
 }
 
 template <typename T>
@@ -270,24 +272,23 @@ struct QuantizeParams {
   FastDivisor by_groups;
 };
 
-// silu(x) = x / (1 + exp(-x)), from z = exp(-|x|) <= 1: x (x < 0 ? z : 1) / (1 + z), which neither overflows
-// nor cancels. z = 2^(hi + lo), hi the rounded and lo the lost part of -|x| log2(e), so that far from zero the
-// exponent's rounding does not show; 1 / (1 + z) by one Newton-Raphson step on the hardware's estimate.
-// Relative error below 10 * 2^-24: the estimate of 2^hi 4, its correction 1, the sum 1, its reciprocal 2, the
-// products 2.
+// silu(x) = x / (1 + exp(-x)) with exp(-x) = 2^-(p + l), p the product x log2(e) rounded down and l >= 0 what
+// that lost: 2^-l = 1 - l ln(2) to the last bit, so that far from zero the exponent's rounding does not show.
+// Where exp(-x) is 2^126 or more (x below -87.3) the result is -0: the estimates' forms without subnormals are
+// four instructions shorter each. Relative error below 9 * 2^-24: the
+// estimate of 2^-p 4, its correction 1, the sum 1, the estimate of its reciprocal 2, the product 1. No
+// comparison or selection: the integer pipe is what bounds the gated kernel.
 __device__ __forceinline__ float silu(float x) {
   constexpr float kLog2e = 1.44269502f, kLog2eRest = 1.92596303e-8f;  // their sum is log2(e) to 2^-49
   constexpr float kLn2 = 0.693147182f;
-  const float a = fminf(fabsf(x), 128.f);  // exp(-128) is zero in f32; a NaN comes back with the factor x
-  const float hi = -a * kLog2e;
-  const float lo = fmaf(-a, kLog2eRest, fmaf(-a, kLog2e, -hi));
-  float z, y;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(z) : "f"(hi));
-  z = fmaf(z, lo * kLn2, z);
-  const float d = 1.f + z;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(y) : "f"(d));
-  y = fmaf(y, fmaf(-d, y, 1.f), y);
-  return x * (x < 0.f ? z : 1.f) * y;
+  const float p = __fmul_rd(x, kLog2e);
+  float lost, e, y;
+  // Saturating: no more than a guard for x log2(e) beyond f32, where p and the difference are not numbers.
+  asm("fma.rn.sat.f32 %0, %1, %2, %3;" : "=f"(lost) : "f"(x), "f"(kLog2e), "f"(-p));
+  const float correction = fmaf(x, -kLog2eRest * kLn2, fmaf(lost, -kLn2, 1.f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-p));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(fmaf(e, correction, 1.f)));
+  return x * y;
 }
 
 // A lane takes UNROLL groups that are 32 apart, so that a block's groups lie next to each other and every
@@ -331,16 +332,20 @@ __global__ void __launch_bounds__(kQuantThreads) cake_quantize_rows_sm100(const 
     F2 v[kLaneVecs][kVec / 2];
     uint32_t a = 0;
     if (GATE) {
+      float magnitude = 0.f;
 #pragma unroll
       for (int k = 0; k < kLaneVecs; ++k)
 #pragma unroll
         for (int i = 0; i < kVec / 2; ++i) {
-          float lo, hi;
-          unpack2(widen<T>(x[u][k], i), lo, hi);
-          v[k][i] = mul2(pack2(silu(lo), silu(hi)), widen<T>(up[GATE ? u : 0][k], i));
-          a = largest(a, v[k][i]);
+          float x0, x1, u0, u1;
+          unpack2(widen<T>(x[u][k], i), x0, x1);
+          unpack2(widen<T>(up[GATE ? u : 0][k], i), u0, u1);
+          x0 = silu(x0) * u0;
+          x1 = silu(x1) * u1;
+          v[k][i] = pack2(x0, x1);
+          magnitude = largest_abs(magnitude, v[k][i]);
         }
-      a = group_max(a);
+      a = group_max(__float_as_uint(magnitude));
     } else {
 #pragma unroll
       for (int k = 0; k < kLaneVecs; ++k) a = largest_raw<T>(a, x[u][k]);
@@ -444,7 +449,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
   const float scale = 1.f / sqrtf(sum / static_cast<float>(p.cols) + p.epsilon);
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
-    uint32_t a = 0;
+    float magnitude = 0.f;
 #pragma unroll
     for (int k = 0; k < kLaneVecs; ++k) {
       const int col = col_of(i) + k * kGroupLanes * kVec;
@@ -453,10 +458,10 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
 #pragma unroll
       for (int e = 0; e < kVec / 2; ++e) {
         h[i][k][e] = mul2(mul2(h[i][k][e], pack2(scale, scale)), widen<W>(weight, e));
-        a = largest(a, h[i][k][e]);
+        magnitude = largest_abs(magnitude, h[i][k][e]);
       }
     }
-    const uint32_t byte = scale_byte(group_max(a));
+    const uint32_t byte = scale_byte(group_max(__float_as_uint(magnitude)));
     const float inverse = inverse_scale(byte);
 #pragma unroll
     for (int k = 0; k < kLaneVecs; ++k) {
