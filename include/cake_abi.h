@@ -319,32 +319,26 @@ int32_t cake_rms_norm_quantize_enqueue(const void* x, int32_t dtype, int64_t x_r
                                        void* scales, int64_t scales_row_stride, void* stream);
 
 /* out[m, n] = sum over k of lhs[m, k] * s_lhs[m, k / 128] * rhs[n, k] * s_rhs[n, k / 128], accumulated in
- * f32 and rounded once to out_dtype. One plan serves any number of rows m. */
+ * f32 and rounded once to out_dtype. */
 typedef struct cake_scaled_matmul_desc {
   int64_t n;         /* rows of rhs = columns of out */
   int64_t k;         /* contraction */
   int32_t out_dtype; /* CAKE_DTYPE_F32 or CAKE_DTYPE_BF16 */
-  int32_t tile;      /* 0 = library default; 128, 192, 224: columns of a 128-row output tile;
+  int32_t tile;      /* 0 = library default; 128, 192, 224, 256: columns of a 256-row output tile;
                         16, 32, 64: tokens of a tile of 128 rhs rows (few rows m) */
   int32_t k_split;   /* 0 = library default; with tile 16, 32 or 64: 1..8 blocks share a tile's contraction */
-  int32_t reserved;  /* 0 */
 } cake_scaled_matmul_desc;
 
-typedef struct cake_scaled_matmul cake_scaled_matmul;
-
-int32_t cake_scaled_matmul_create(const cake_scaled_matmul_desc* desc, cake_scaled_matmul** out);
-int32_t cake_scaled_matmul_destroy(cake_scaled_matmul* plan);
-
-/* lhs [m, k], rhs [n, k]: codes, 16-byte aligned with row strides that are multiples of 16 bytes;
- * scales: any alignment and row stride; out: [m, n], aligned to its elements, any row stride (elements).
- * m may be 0. Uses no workspace. */
-int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const void* lhs, int64_t lhs_row_stride,
-                                   const void* lhs_scales, int64_t lhs_scales_row_stride, const void* rhs,
-                                   int64_t rhs_row_stride, const void* rhs_scales, int64_t rhs_scales_row_stride,
-                                   void* out, int64_t out_row_stride, void* stream);
-
-/* Reads (and clears) the device status word; synchronises the stream first. */
-int32_t cake_scaled_matmul_status(cake_scaled_matmul* plan, void* stream, cake_status* out);
+/* lhs [m, k], rhs [n, k]: codes, 16-byte aligned with row strides that are multiples of 16 bytes (of 128:
+ * faster); scales: any alignment and row stride; out: [m, n], aligned to its elements, any row stride
+ * (elements). m may be 0. There is no handle, no workspace and nothing kept between calls: calls may
+ * overlap on the GPU. status_device: optional 4 int32 in device memory, zeroed by the caller, that receive
+ * the cake_status fields if a bounded wait runs out (code 1: the output is not valid); NULL to ignore. */
+int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t m, const void* lhs,
+                                   int64_t lhs_row_stride, const void* lhs_scales, int64_t lhs_scales_row_stride,
+                                   const void* rhs, int64_t rhs_row_stride, const void* rhs_scales,
+                                   int64_t rhs_scales_row_stride, void* out, int64_t out_row_stride,
+                                   int32_t* status_device, void* stream);
 
 #ifdef __cplusplus
 }

@@ -81,7 +81,7 @@ def test_quantize_is_exact(cuda_device, dtype, rows, cols, pad):
     plan = scaled.CudaQuantizeRowsPlan(name="t", columns=cols, input_dtype=dtype)
     codes, scales = plan.invoke(plan.build(cuda_device), x)
     expected_codes, expected_scales = oracle.quantize(numpy64(x))
-    assert codes.stride(0) % 16 == 0
+    assert codes.stride(0) % 128 == 0
     assert np.array_equal(numpy64(codes), expected_codes)
     assert np.array_equal(scale_values(scales), expected_scales)
 
@@ -202,7 +202,7 @@ def run_matmul(device, m, n, k, *, seed=0, exact=True, output_dtype="f32", tile=
     return out, a @ b.T, np.abs(a) @ np.abs(b).T
 
 
-@pytest.mark.parametrize("tile, k_split", [(16, 1), (16, 2), (16, 3), (16, 8), (32, 1), (32, 4), (64, 1), (64, 2), (128, 0), (192, 0), (224, 0), (0, 0)])
+@pytest.mark.parametrize("tile, k_split", [(16, 1), (16, 2), (16, 3), (16, 8), (32, 1), (32, 4), (64, 1), (64, 2), (128, 0), (192, 0), (224, 0), (256, 0), (0, 0)])
 @pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 128, 128), (16, 128, 1024), (5, 300, 520), (33, 129, 650), (130, 225, 140), (200, 448, 2048)])
 def test_matmul_is_exact_where_f32_is(cuda_device, m, n, k, tile, k_split):
     # Codes -3..3 and scales 1/2, 1, 2: sums of multiples of 1/4 below 36 k, which f32 holds exactly.
@@ -382,6 +382,3 @@ def test_entry_points_refuse_what_tensor_maps_cannot_hold(cuda_device):
         plan.invoke(executable, lhs, lhs_scales, bad_base, lhs_scales)
     with pytest.raises(ValueError, match="must be on"):
         plan.invoke(executable, lhs.cpu(), lhs_scales, lhs, lhs_scales)
-    executable.close()
-    with pytest.raises(RuntimeError, match="closed"):
-        plan.invoke(executable, lhs, lhs_scales, lhs, lhs_scales)

@@ -49,7 +49,7 @@ def test_plans_refuse_what_they_do_not_run():
         with pytest.raises(ValueError):
             scaled.CudaRmsNormQuantizePlan(name="p", **arguments)
     for arguments in ({"n": 0, "k": 8}, {"n": 8, "k": 0}, {"n": 1 << 30, "k": 8}, {"n": 8, "k": 8, "output_dtype": "f16"},
-                      {"n": 8, "k": 8, "tile": 256}, {"n": 8, "k": 8, "k_split": 2}, {"n": 8, "k": 8, "tile": 128, "k_split": 2},
+                      {"n": 8, "k": 8, "tile": 160}, {"n": 8, "k": 8, "tile": 256, "k_split": 2}, {"n": 8, "k": 8, "k_split": 2}, {"n": 8, "k": 8, "tile": 128, "k_split": 2},
                       {"n": 8, "k": 8, "tile": 16, "k_split": 9}):
         with pytest.raises(ValueError):
             scaled.CudaScaledMatmulPlan(name="p", **arguments)
@@ -64,7 +64,7 @@ def test_plan_sources_tell_plans_apart():
     assert "cake_quantize_rows_sm100" in scaled.CudaQuantizeRowsPlan(name="p", columns=64).render_executable_source()
 
 
-@pytest.mark.parametrize("columns, pitch", [(1, 16), (16, 16), (100, 112), (128, 128), (1000, 1008)])
+@pytest.mark.parametrize("columns, pitch", [(1, 128), (16, 128), (100, 128), (128, 128), (1000, 1024)])
 def test_codes_get_the_pitch_the_matmul_wants(columns, pitch):
     codes = scaled.empty_codes(3, columns, torch.device("cpu"))
     assert tuple(codes.shape) == (3, columns) and codes.stride() == (pitch, 1) and codes.dtype == torch.float8_e4m3fn
@@ -187,29 +187,42 @@ def test_norm_refuses_bad_arguments(overrides, code, fragment):
     assert fragment in _native.load().cake_last_error().decode()
 
 
+def _matmul(**overrides):
+    desc = dict(n=128, k=128, out_dtype=1, tile=0, k_split=0)
+    arguments = dict(m=2, lhs=1 << 20, lhs_stride=128, lhs_scales=1 << 20, lhs_scales_stride=1, rhs=1 << 20, rhs_stride=128, rhs_scales=1 << 20,
+                     rhs_scales_stride=1, out=1 << 20, out_stride=128, status=None, stream=None)
+    for name, value in overrides.items():
+        (desc if name in desc else arguments)[name] = value
+    return _native.load().cake_scaled_matmul_enqueue(ctypes.byref(_native.ScaledMatmulDesc(**desc)), *arguments.values())
+
+
 @pytest.mark.parametrize("overrides, code, fragment", [
     ({"n": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
     ({"k": 1 << 31}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
     ({"out_dtype": 2}, _native.CAKE_ERR_INVALID_ARGUMENT, "out_dtype"),
-    ({"tile": 256}, _native.CAKE_ERR_UNSUPPORTED, "tile"),
+    ({"tile": 160}, _native.CAKE_ERR_UNSUPPORTED, "tile"),
     ({"k_split": 9, "tile": 16}, _native.CAKE_ERR_INVALID_ARGUMENT, "k_split"),
     ({"k_split": 2}, _native.CAKE_ERR_INVALID_ARGUMENT, "k_split"),
     ({"k_split": 2, "tile": 224}, _native.CAKE_ERR_INVALID_ARGUMENT, "k_split"),
-    ({"reserved": 1}, _native.CAKE_ERR_INVALID_ARGUMENT, "reserved"),
+    ({"m": -1}, _native.CAKE_ERR_INVALID_ARGUMENT, "m must"),
+    ({"m": 1 << 30}, _native.CAKE_ERR_INVALID_ARGUMENT, "m must"),
+    ({"lhs": None}, _native.CAKE_ERR_INVALID_ARGUMENT, "null"),
+    ({"rhs_scales": None}, _native.CAKE_ERR_INVALID_ARGUMENT, "null"),
+    ({"lhs": (1 << 20) + 8}, _native.CAKE_ERR_INVALID_ARGUMENT, "16-byte aligned"),
+    ({"rhs_stride": 136}, _native.CAKE_ERR_INVALID_ARGUMENT, "multiples of 16"),
+    ({"lhs_stride": 112}, _native.CAKE_ERR_INVALID_ARGUMENT, "at least k"),
+    ({"lhs_scales_stride": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "scales row stride"),
+    ({"rhs_scales_stride": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "scales row stride"),
+    ({"out_stride": 127}, _native.CAKE_ERR_INVALID_ARGUMENT, "output row stride"),
+    ({"out": (1 << 20) + 1}, _native.CAKE_ERR_INVALID_ARGUMENT, "aligned to its elements"),
+    ({"status": (1 << 20) + 2}, _native.CAKE_ERR_INVALID_ARGUMENT, "status_device"),
 ])
-def test_scaled_matmul_refuses_bad_descriptors(overrides, code, fragment):
-    lib = _native.load()
-    fields = dict(n=128, k=128, out_dtype=1, tile=0, k_split=0, reserved=0)
-    fields.update(overrides)
-    handle = ctypes.c_void_p()
-    assert lib.cake_scaled_matmul_create(ctypes.byref(_native.ScaledMatmulDesc(**fields)), ctypes.byref(handle)) == code
-    assert fragment in lib.cake_last_error().decode()
+def test_scaled_matmul_refuses_bad_arguments(overrides, code, fragment):
+    assert _matmul(**overrides) == code
+    assert fragment in _native.load().cake_last_error().decode()
 
 
-def test_null_handles_are_errors_not_crashes():
-    lib = _native.load()
+def test_null_descriptor_is_an_error_and_no_rows_are_no_work():
     assert ctypes.sizeof(_native.ScaledMatmulDesc) == 32
-    assert lib.cake_scaled_matmul_create(None, None) == _native.CAKE_ERR_INVALID_ARGUMENT
-    assert lib.cake_scaled_matmul_enqueue(None, 1, None, 0, None, 0, None, 0, None, 0, None, 0, None) == _native.CAKE_ERR_INVALID_ARGUMENT
-    assert lib.cake_scaled_matmul_status(None, None, None) == _native.CAKE_ERR_INVALID_ARGUMENT
-    assert lib.cake_scaled_matmul_destroy(None) == _native.CAKE_OK
+    assert _native.load().cake_scaled_matmul_enqueue(None, 1, *[None, 0] * 5, None, None) == _native.CAKE_ERR_INVALID_ARGUMENT
+    assert _matmul(m=0, lhs=None, lhs_scales=None, rhs=None, rhs_scales=None, out=None) == _native.CAKE_OK

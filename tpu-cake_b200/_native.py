@@ -66,10 +66,7 @@ EXPORTED_SYMBOLS = (
     "cake_rpa_launches_per_enqueue",
     "cake_quantize_rows_enqueue",
     "cake_rms_norm_quantize_enqueue",
-    "cake_scaled_matmul_create",
-    "cake_scaled_matmul_destroy",
     "cake_scaled_matmul_enqueue",
-    "cake_scaled_matmul_status",
 )
 
 
@@ -138,7 +135,6 @@ class ScaledMatmulDesc(ctypes.Structure):
         ("out_dtype", ctypes.c_int32),
         ("tile", ctypes.c_int32),
         ("k_split", ctypes.c_int32),
-        ("reserved", ctypes.c_int32),
     ]
 
 
@@ -226,14 +222,8 @@ def load() -> ctypes.CDLL:
     lib.cake_quantize_rows_enqueue.argtypes = [vp, i32, i64, i32, i64, i64, vp, i64, vp, i64, vp]
     lib.cake_rms_norm_quantize_enqueue.restype = i32
     lib.cake_rms_norm_quantize_enqueue.argtypes = [vp, i32, i64, vp, i64, vp, i64, vp, i32, ctypes.c_float, i64, i64, vp, i64, vp, i64, vp]
-    lib.cake_scaled_matmul_create.restype = i32
-    lib.cake_scaled_matmul_create.argtypes = [ctypes.POINTER(ScaledMatmulDesc), ctypes.POINTER(vp)]
-    lib.cake_scaled_matmul_destroy.restype = i32
-    lib.cake_scaled_matmul_destroy.argtypes = [vp]
     lib.cake_scaled_matmul_enqueue.restype = i32
-    lib.cake_scaled_matmul_enqueue.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp]
-    lib.cake_scaled_matmul_status.restype = i32
-    lib.cake_scaled_matmul_status.argtypes = [vp, vp, ctypes.POINTER(CakeStatus)]
+    lib.cake_scaled_matmul_enqueue.argtypes = [vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp]
     _lib = lib
     return lib
 

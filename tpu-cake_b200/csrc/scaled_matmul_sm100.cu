@@ -22,8 +22,6 @@
 #include <cuda_bf16.h>
 #include <string.h>
 
-#include <new>
-
 #include "cake_host.h"
 #include "cake_ptx.cuh"
 
@@ -63,7 +61,8 @@ struct Cfg {
   static constexpr int kFit = static_cast<int>((kRoom - kStaging - kScaleSlots * kScaleSlotBytes) / kStageBytes);
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   // Accumulators, then kScaleSets sets of scale columns (4 for A, 4 per 128 rows of B).
-  static constexpr int kAccumulators = NARROW ? 1 : 2;
+  // Two accumulators of 256 columns would leave no room for scales.
+  static constexpr int kAccumulators = NARROW || BN > 224 ? 1 : 2;
   static constexpr int kScaleCols = 4 * (1 + kScaleBlocksB);
   static constexpr int kScaleBase = kAccumulators * BN;
   static constexpr int kTmemCols = pow2_at_least(kScaleBase + kScaleSets * kScaleCols);
@@ -334,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
     constexpr uint32_t kIdesc = umma_idesc_mxf8(PAIR ? 2 * kRowsA : kRowsA, BN, 0);
     uint32_t stage = 0, phase = 0, set = 0, set_phase = 0;
     int it = 0;
-    bool ok = true;
+    bool ok = true, ready = false;  // ready: the next k block's operands have been seen to be there
     for (int t = first_tile; t < num_tiles && ok; t += tile_step, ++it) {
       const int buf = C::kAccumulators == 2 ? (it & 1) : 0;
       const uint32_t acc_phase = C::kAccumulators == 2 ? ((it >> 1) & 1) : (it & 1);
@@ -357,13 +356,15 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
 #pragma unroll
         for (int byte = 0; byte < 4; ++byte) {
           if (kb + byte >= kb_end) break;
-          if (!wait_warp<false>(smem_u32(&full_bar[stage]), phase, abort_flag)) {
+          if (!ready && !wait_warp<false>(smem_u32(&full_bar[stage]), phase, abort_flag)) {
             if (!*abort_flag && issuer) record(p.status, 1, blockIdx.x, t, 300 + stage);
             *abort_flag = 1;
             ok = false;
             break;
           }
           tcgen05_fence_after();
+          const uint32_t next_stage = stage + 1 == STAGES ? 0 : stage + 1, next_phase = next_stage == 0 ? phase ^ 1 : phase;
+          const bool seen = mbar_test_wait(smem_u32(&full_bar[next_stage]), next_phase);  // answers while MMAs are issued
           if (issuer) {
             const uint64_t a_desc = desc0 + stage * kStageStep;
             const uint64_t b_desc = a_desc + (C::kABytes >> 4);
@@ -379,10 +380,9 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
             commit<PAIR>(smem_u32(&empty_bar[stage]));
           }
           accumulate = 1;
-          if (++stage == STAGES) {
-            stage = 0;
-            phase ^= 1;
-          }
+          ready = __all_sync(0xffffffffu, seen);
+          stage = next_stage;
+          phase = next_phase;
         }
         if (ok && issuer) tcgen05_commit_as<PAIR>(smem_u32(&set_empty[set]));
         if (++set == kScaleSets) {
@@ -655,28 +655,43 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
 
 // ====================================================================================== host
 
-struct cake_scaled_matmul {
-  cake_scaled_matmul_desc d;
-  int device = 0;
-  int sm_count = 0;
-  cake::StatusWord status;
-};
-
 namespace {
 
 using cake::fail;
 
+// What a launch has to know about the current device, looked up once per device.
+struct Device {
+  int index = -1;
+  int sm_count = 0;
+};
+
+int32_t current_device(Device* d) {
+  static int sm_counts[64] = {};
+  CAKE_CUDA_TRY(cudaGetDevice(&d->index));
+  const bool cached = d->index >= 0 && d->index < 64;
+  if (cached && sm_counts[d->index] > 0) {
+    d->sm_count = sm_counts[d->index];
+    return CAKE_OK;
+  }
+  int major = 0;
+  CAKE_CUDA_TRY(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, d->index));
+  if (major != 10) return fail(CAKE_ERR_UNSUPPORTED, "libcake_b200 needs an sm_100 GPU, found compute capability %d.x", major);
+  CAKE_CUDA_TRY(cudaDeviceGetAttribute(&d->sm_count, cudaDevAttrMultiProcessorCount, d->index));
+  if (cached) sm_counts[d->index] = d->sm_count;
+  return CAKE_OK;
+}
+
 template <int BN, bool NARROW>
-int32_t launch(const cake_scaled_matmul* plan, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out,
+int32_t launch(const Device& device, const CUtensorMap& a, const CUtensorMap& b, const CUtensorMap& out,
                const cake::Params& p, cudaStream_t stream) {
   using C = cake::Cfg<BN, NARROW>;
   auto kernel = cake::cake_scaled_matmul_sm100<BN, NARROW>;
   // The opt-in to more than 48 KB of dynamic shared memory is a per-device attribute.
   static bool configured[64] = {};
-  const int slot = plan->device >= 0 && plan->device < 64 ? plan->device : 0;
-  if (!configured[slot]) {
+  const bool cached = device.index >= 0 && device.index < 64;
+  if (!cached || !configured[device.index]) {
     CAKE_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmemBytes));
-    configured[slot] = plan->device >= 0 && plan->device < 64;
+    if (cached) configured[device.index] = true;
   }
   const int64_t tiles = static_cast<int64_t>(p.tiles_a) * p.tiles_b;
   cudaLaunchAttribute attrs[2];
@@ -687,7 +702,7 @@ int32_t launch(const cake_scaled_matmul* plan, const CUtensorMap& a, const CUten
   attrs[1].val.clusterDim.y = 1;
   attrs[1].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(NARROW ? tiles * p.split : 2 * (tiles < plan->sm_count / 2 ? tiles : plan->sm_count / 2)));
+  config.gridDim = dim3(static_cast<unsigned>(NARROW ? tiles * p.split : 2 * (tiles < device.sm_count / 2 ? tiles : device.sm_count / 2)));
   config.blockDim = dim3(cake::kThreads);
   config.dynamicSmemBytes = C::kSmemBytes;
   config.stream = stream;
@@ -711,8 +726,7 @@ struct Choice {
 
 bool is_narrow(int tile) { return tile <= 64; }
 
-Choice choose(const cake_scaled_matmul* plan, int64_t m) {
-  const cake_scaled_matmul_desc& d = plan->d;
+Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count) {
   Choice c = {d.tile, d.k_split};
   const int64_t k_blocks = (d.k + cake::kBlockK - 1) / cake::kBlockK;
   if (c.tile == 0) {
@@ -721,10 +735,13 @@ Choice choose(const cake_scaled_matmul* plan, int64_t m) {
     else if (m <= 256) c.tile = 64;
     else {
       int64_t best = 0;
-      for (int tile : {128, 192, 224}) {
+      const int64_t pairs = sm_count / 2;
+      for (int tile : {128, 192, 224, 256}) {
         const int64_t tiles = ((m + 255) / 256) * ((d.n + tile - 1) / tile);
-        const int64_t pairs = plan->sm_count / 2;
-        const int64_t cost = (tiles + pairs - 1) / pairs * tile;
+        const int64_t waves = (tiles + pairs - 1) / pairs;
+        // Cycles: a k block takes 2 tile, but not less than 400; an epilogue that nothing hides 16 a column.
+        const int64_t k_block = 2 * tile > 400 ? 2 * tile : 400;
+        const int64_t cost = waves * k_blocks * k_block + (tile == 256 ? waves : 1) * 16 * tile;
         if (best == 0 || cost <= best) {
           best = cost;
           c.tile = tile;
@@ -736,7 +753,7 @@ Choice choose(const cake_scaled_matmul* plan, int64_t m) {
   else if (c.split == 0) {
     const int64_t tiles = ((d.n + 127) / 128) * ((m + c.tile - 1) / c.tile);
     c.split = 1;
-    while (c.split < 8 && 2 * c.split * tiles <= plan->sm_count && 2 * c.split <= k_blocks) c.split *= 2;
+    while (c.split < 8 && 2 * c.split * tiles <= sm_count && 2 * c.split <= k_blocks) c.split *= 2;
   }
   if (c.split > k_blocks) c.split = static_cast<int>(k_blocks);
   return c;
@@ -746,56 +763,21 @@ Choice choose(const cake_scaled_matmul* plan, int64_t m) {
 
 extern "C" {
 
-int32_t cake_scaled_matmul_create(const cake_scaled_matmul_desc* desc, cake_scaled_matmul** out) {
-  if (!desc || !out) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_create: null argument");
+int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t m, const void* lhs, int64_t lhs_row_stride,
+                                   const void* lhs_scales, int64_t lhs_scales_row_stride, const void* rhs,
+                                   int64_t rhs_row_stride, const void* rhs_scales, int64_t rhs_scales_row_stride,
+                                   void* out, int64_t out_row_stride, int32_t* status_device, void* stream) {
+  if (!desc) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_enqueue: null argument");
   const cake_scaled_matmul_desc& d = *desc;
   // Rows and columns are tensor-map coordinates; a tile past the end must not wrap around either.
   if (d.n < 1 || d.k < 1 || d.n > INT32_MAX / 2 || d.k > INT32_MAX / 2)
     return fail(CAKE_ERR_INVALID_ARGUMENT, "scaled matmul extents must be 1 to 2^30 - 1: n=%lld k=%lld", (long long)d.n, (long long)d.k);
   if (d.out_dtype != CAKE_DTYPE_F32 && d.out_dtype != CAKE_DTYPE_BF16)
     return fail(CAKE_ERR_INVALID_ARGUMENT, "out_dtype must be CAKE_DTYPE_F32 or CAKE_DTYPE_BF16");
-  if (d.tile != 0 && d.tile != 16 && d.tile != 32 && d.tile != 64 && d.tile != 128 && d.tile != 192 && d.tile != 224)
-    return fail(CAKE_ERR_UNSUPPORTED, "tile must be 0, 16, 32, 64, 128, 192 or 224, got %d", d.tile);
-  if (d.k_split < 0 || d.k_split > 8 || (d.k_split > 1 && !is_narrow(d.tile)) || (d.k_split > 1 && d.tile == 0))
+  if (d.tile != 0 && d.tile != 16 && d.tile != 32 && d.tile != 64 && d.tile != 128 && d.tile != 192 && d.tile != 224 && d.tile != 256)
+    return fail(CAKE_ERR_UNSUPPORTED, "tile must be 0, 16, 32, 64, 128, 192, 224 or 256, got %d", d.tile);
+  if (d.k_split < 0 || d.k_split > 8 || (d.k_split > 1 && (!is_narrow(d.tile) || d.tile == 0)))
     return fail(CAKE_ERR_INVALID_ARGUMENT, "k_split must be 0 to 8, and above 1 only with tile 16, 32 or 64, got %d", d.k_split);
-  if (d.reserved != 0) return fail(CAKE_ERR_INVALID_ARGUMENT, "reserved must be 0");
-  cake_scaled_matmul* plan = new (std::nothrow) cake_scaled_matmul();
-  if (!plan) return fail(CAKE_ERR_CUDA, "out of host memory");
-  plan->d = d;
-  cudaError_t e = cudaGetDevice(&plan->device);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&plan->sm_count, cudaDevAttrMultiProcessorCount, plan->device);
-  int major = 0;
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, plan->device);
-  if (e != cudaSuccess) {
-    delete plan;
-    return fail(CAKE_ERR_CUDA, "no usable CUDA device: %s", cudaGetErrorString(e));
-  }
-  if (major != 10) {
-    delete plan;
-    return fail(CAKE_ERR_UNSUPPORTED, "libcake_b200 needs an sm_100 GPU, found compute capability %d.x", major);
-  }
-  const int32_t rc = plan->status.ensure();
-  if (rc != CAKE_OK) {
-    cake_scaled_matmul_destroy(plan);
-    return rc;
-  }
-  *out = plan;
-  return CAKE_OK;
-}
-
-int32_t cake_scaled_matmul_destroy(cake_scaled_matmul* plan) {
-  if (!plan) return CAKE_OK;
-  plan->status.release();
-  delete plan;
-  return CAKE_OK;
-}
-
-int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const void* lhs, int64_t lhs_row_stride,
-                                   const void* lhs_scales, int64_t lhs_scales_row_stride, const void* rhs,
-                                   int64_t rhs_row_stride, const void* rhs_scales, int64_t rhs_scales_row_stride,
-                                   void* out, int64_t out_row_stride, void* stream) {
-  if (!plan) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_enqueue: null argument");
-  const cake_scaled_matmul_desc& d = plan->d;
   if (m < 0 || m > INT32_MAX / 2) return fail(CAKE_ERR_INVALID_ARGUMENT, "m must be 0 to 2^30 - 1, got %lld", (long long)m);
   if (m == 0) return CAKE_OK;
   if (!lhs || !lhs_scales || !rhs || !rhs_scales || !out) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_enqueue: null argument");
@@ -818,7 +800,12 @@ int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const vo
   if (out_row_stride < d.n) return fail(CAKE_ERR_INVALID_ARGUMENT, "the output row stride is shorter than its row");
   if (reinterpret_cast<uintptr_t>(out) % osize) return fail(CAKE_ERR_INVALID_ARGUMENT, "out is not aligned to its elements");
 
-  const Choice c = choose(plan, m);
+  if (reinterpret_cast<uintptr_t>(status_device) & 3) return fail(CAKE_ERR_INVALID_ARGUMENT, "status_device must be 4-byte aligned");
+
+  Device device;
+  int32_t rc = current_device(&device);
+  if (rc) return rc;
+  const Choice c = choose(d, m, device.sm_count);
   const bool narrow = is_narrow(c.tile);
   cake::Params p;
   memset(&p, 0, sizeof(p));
@@ -841,14 +828,14 @@ int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const vo
   p.scales_b_stride = narrow ? lhs_scales_row_stride : rhs_scales_row_stride;
   p.out = out;
   p.out_stride = out_row_stride;
-  p.status = plan->status.dev;
+  p.status = status_device;
   // Tensor stores write whole 16-byte pieces, also where the row ends inside one: only rows of whole pieces
   // leave what lies behind them alone.
   p.tma_store = !narrow && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && out_row_stride * osize % 16 == 0 && d.n * osize % 16 == 0;
 
   CUtensorMap map_a, map_b, map_out;
   memset(&map_out, 0, sizeof(map_out));
-  int32_t rc = encode_operand(&map_a, narrow ? rhs : lhs, rows_a, d.k, narrow ? rhs_row_stride : lhs_row_stride, cake::kRowsA);
+  rc = encode_operand(&map_a, narrow ? rhs : lhs, rows_a, d.k, narrow ? rhs_row_stride : lhs_row_stride, cake::kRowsA);
   if (rc) return rc;
   rc = encode_operand(&map_b, narrow ? lhs : rhs, rows_b, d.k, narrow ? lhs_row_stride : rhs_row_stride, narrow ? c.tile : c.tile / 2);
   if (rc) return rc;
@@ -862,22 +849,14 @@ int32_t cake_scaled_matmul_enqueue(cake_scaled_matmul* plan, int64_t m, const vo
   }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (c.tile) {
-    case 16: return launch<16, true>(plan, map_a, map_b, map_out, p, s);
-    case 32: return launch<32, true>(plan, map_a, map_b, map_out, p, s);
-    case 64: return launch<64, true>(plan, map_a, map_b, map_out, p, s);
-    case 128: return launch<128, false>(plan, map_a, map_b, map_out, p, s);
-    case 192: return launch<192, false>(plan, map_a, map_b, map_out, p, s);
-    default: return launch<224, false>(plan, map_a, map_b, map_out, p, s);
+    case 16: return launch<16, true>(device, map_a, map_b, map_out, p, s);
+    case 32: return launch<32, true>(device, map_a, map_b, map_out, p, s);
+    case 64: return launch<64, true>(device, map_a, map_b, map_out, p, s);
+    case 128: return launch<128, false>(device, map_a, map_b, map_out, p, s);
+    case 192: return launch<192, false>(device, map_a, map_b, map_out, p, s);
+    case 224: return launch<224, false>(device, map_a, map_b, map_out, p, s);
+    default: return launch<256, false>(device, map_a, map_b, map_out, p, s);
   }
-}
-
-int32_t cake_scaled_matmul_status(cake_scaled_matmul* plan, void* stream, cake_status* out) {
-  if (!plan || !out) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_status: null argument");
-  const int32_t rc = plan->status.read_and_clear(static_cast<cudaStream_t>(stream), out);
-  if (rc) return rc;
-  if (out->code == 1)
-    return fail(CAKE_ERR_TIMEOUT, "device-side bounded wait ran out: block=%d tile=%d where=%d", out->detail0, out->detail1, out->detail2);
-  return CAKE_OK;
 }
 
 }  // extern "C"
