@@ -324,9 +324,9 @@ typedef struct cake_scaled_matmul_desc {
   int64_t n;         /* rows of rhs = columns of out */
   int64_t k;         /* contraction */
   int32_t out_dtype; /* CAKE_DTYPE_F32 or CAKE_DTYPE_BF16 */
-  int32_t tile;      /* 0 = library default; 128, 192, 224, 256: columns of a 256-row output tile;
-                        16, 32, 64: tokens of a tile of 128 rhs rows (few rows m) */
-  int32_t k_split;   /* 0 = library default; with tile 16, 32 or 64: 1..8 blocks share a tile's contraction */
+  int32_t tile;      /* 0 = library default; 192, 224, 256: columns of a 256-row output tile;
+                        16, 32, 64, 128: tokens of a tile of 128 rhs rows (few rows m) */
+  int32_t k_split;   /* 0 = library default; with tile 16 to 128: 1..8 blocks share a tile's contraction */
 } cake_scaled_matmul_desc;
 
 /* lhs [m, k], rhs [n, k]: codes, 16-byte aligned with row strides that are multiples of 16 bytes (of 128:

@@ -202,7 +202,7 @@ def run_matmul(device, m, n, k, *, seed=0, exact=True, output_dtype="f32", tile=
     return out, a @ b.T, np.abs(a) @ np.abs(b).T
 
 
-@pytest.mark.parametrize("tile, k_split", [(16, 1), (16, 2), (16, 3), (16, 8), (32, 1), (32, 4), (64, 1), (64, 2), (128, 0), (192, 0), (224, 0), (256, 0), (0, 0)])
+@pytest.mark.parametrize("tile, k_split", [(16, 1), (16, 2), (16, 3), (16, 8), (32, 1), (32, 4), (64, 1), (64, 2), (128, 1), (128, 5), (192, 0), (224, 0), (256, 0), (0, 0)])
 @pytest.mark.parametrize("m, n, k", [(1, 1, 1), (1, 128, 128), (16, 128, 1024), (5, 300, 520), (33, 129, 650), (130, 225, 140), (200, 448, 2048)])
 def test_matmul_is_exact_where_f32_is(cuda_device, m, n, k, tile, k_split):
     # Codes -3..3 and scales 1/2, 1, 2: sums of multiples of 1/4 below 36 k, which f32 holds exactly.

@@ -49,7 +49,7 @@ def test_plans_refuse_what_they_do_not_run():
         with pytest.raises(ValueError):
             scaled.CudaRmsNormQuantizePlan(name="p", **arguments)
     for arguments in ({"n": 0, "k": 8}, {"n": 8, "k": 0}, {"n": 1 << 30, "k": 8}, {"n": 8, "k": 8, "output_dtype": "f16"},
-                      {"n": 8, "k": 8, "tile": 160}, {"n": 8, "k": 8, "tile": 256, "k_split": 2}, {"n": 8, "k": 8, "k_split": 2}, {"n": 8, "k": 8, "tile": 128, "k_split": 2},
+                      {"n": 8, "k": 8, "tile": 160}, {"n": 8, "k": 8, "tile": 256, "k_split": 2}, {"n": 8, "k": 8, "k_split": 2}, {"n": 8, "k": 8, "tile": 192, "k_split": 2},
                       {"n": 8, "k": 8, "tile": 16, "k_split": 9}):
         with pytest.raises(ValueError):
             scaled.CudaScaledMatmulPlan(name="p", **arguments)

@@ -22,6 +22,9 @@
 #include <cuda_bf16.h>
 #include <string.h>
 
+#include <algorithm>
+#include <cmath>
+
 #include "cake_host.h"
 #include "cake_ptx.cuh"
 
@@ -105,10 +108,9 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, vol
   }
 }
 
-// The scale bytes of COUNT operand rows for 16 k blocks, from k block kb on, as four words each; 127 (the
-// number 1) past the end. `align`: the rows' addresses and kb are multiples of it (16, 4 or 1). Every branch
-// is the whole warp's and has all rows' loads inside, so that they are under way together: with a branch
-// around each load they ran one after another, and the scales of a word came later than its four k blocks.
+// The scale bytes of COUNT operand rows for 16 k blocks, from k block kb on, as four words each; anything past
+// the last k block. `align`: the rows' addresses and kb are multiples of it (16, 4 or 1). Every branch is the
+// whole warp's and has all rows' loads inside, so that they are under way together.
 template <int COUNT>
 __device__ __forceinline__ void load_scales(uint32_t (&w)[COUNT][4], const uint8_t* const (&row)[COUNT], int kb, int k_blocks, int align) {
   if (align == 16 && kb + 16 <= k_blocks) {
@@ -128,16 +130,17 @@ __device__ __forceinline__ void load_scales(uint32_t (&w)[COUNT][4], const uint8
     if (align >= 4 && at + 4 <= k_blocks) {
 #pragma unroll
       for (int r = 0; r < COUNT; ++r) w[r][i] = __ldg(reinterpret_cast<const uint32_t*>(row[r] + at));
+    } else if (at < k_blocks) {
+      uint32_t byte[COUNT][4];
+#pragma unroll
+      for (int r = 0; r < COUNT; ++r)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) byte[r][j] = __ldg(row[r] + min(at + j, k_blocks - 1));
+#pragma unroll
+      for (int r = 0; r < COUNT; ++r) w[r][i] = byte[r][0] | (byte[r][1] << 8) | (byte[r][2] << 16) | (byte[r][3] << 24);
     } else {
 #pragma unroll
       for (int r = 0; r < COUNT; ++r) w[r][i] = 0x7F7F7F7Fu;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (at + j < k_blocks) {
-#pragma unroll
-          for (int r = 0; r < COUNT; ++r) w[r][i] ^= (0x7Fu ^ __ldg(row[r] + at + j)) << (8 * j);
-        }
-      }
     }
   }
 }
@@ -173,6 +176,64 @@ __device__ __forceinline__ bool wait_or_abort_cluster(uint32_t bar, uint32_t par
       if (mbar_try_wait_cluster(bar, parity)) return true;
     if (*abort_flag) return false;
     if (clock64() - start > kBudgetCycles) return false;
+  }
+}
+
+__device__ __forceinline__ void store_as(char* at, uint32_t v, float) { *reinterpret_cast<uint32_t*>(at) = v; }
+__device__ __forceinline__ void store_as(char* at, uint32_t v, __nv_bfloat16) { *reinterpret_cast<__nv_bfloat16*>(at) = __float2bfloat16_rn(__uint_as_float(v)); }
+
+// One column of up to 16 tokens.
+template <typename T>
+__device__ __forceinline__ void store_tokens(char* at, int64_t stride, const uint32_t (&v)[16], int tokens) {
+  if (tokens >= 16) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j, at += stride) store_as(at, v[j], T());
+  } else {
+#pragma unroll
+    for (int j = 0; j < 16; ++j, at += stride)
+      if (j < tokens) store_as(at, v[j], T());
+  }
+}
+
+// This block's share of a tile's pieces (one token, four columns): the sums over the cluster's blocks in rank
+// order. Distributed shared memory answers slowly, so a thread has up to BLOCKS * AHEAD loads under way.
+template <int BLOCKS, int AHEAD>
+__device__ __forceinline__ void reduce_pieces(const Params& p, uint32_t base, int rank, int col0, int token0, int pieces) {
+  const int step = p.split * kThreads;
+  for (int first = rank * kThreads + static_cast<int>(threadIdx.x); first < pieces; first += AHEAD * step) {
+    float4 v[AHEAD][BLOCKS];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = first + a * step;
+      if (i < pieces) {
+        const uint32_t at = base + ((i / (kRowsA / 4)) * kReducePitch + (i % (kRowsA / 4)) * 4) * 4;
+#pragma unroll
+        for (int s = 0; s < BLOCKS; ++s) v[a][s] = s < p.split ? ld_cluster_f32x4(at, s) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+    }
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int i = first + a * step;
+      if (i >= pieces) break;
+      float4 sum = v[a][0];
+#pragma unroll
+      for (int s = 1; s < BLOCKS; ++s) {
+        sum.x += v[a][s].x;
+        sum.y += v[a][s].y;
+        sum.z += v[a][s].z;
+        sum.w += v[a][s].w;
+      }
+      const float e[4] = {sum.x, sum.y, sum.z, sum.w};
+      const int col = col0 + (i % (kRowsA / 4)) * 4;
+      const int64_t dst = static_cast<int64_t>(token0 + i / (kRowsA / 4)) * p.out_stride + col;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (col + j < p.rows_a) {
+          if (p.out_f32) static_cast<float*>(p.out)[dst + j] = e[j];
+          else static_cast<__nv_bfloat16*>(p.out)[dst + j] = __float2bfloat16_rn(e[j]);
+        }
+      }
+    }
   }
 }
 
@@ -441,24 +502,21 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
     // 16 k blocks at a time: the fence and the arrival at cluster scope take some 1500 cycles, which a word
     // at a time was more than its four k blocks' MMAs. Rows past an operand's end (and past the tile's)
     // get the last row's scales: their codes are zeros, or not there, and what comes of them is not stored.
-    const int align_a = scale_alignment(p.scales_a, p.scales_a_stride, kb_begin);
-    const int align_b = scale_alignment(p.scales_b, p.scales_b_stride, kb_begin);
+    const int align = min(scale_alignment(p.scales_a, p.scales_a_stride, kb_begin), scale_alignment(p.scales_b, p.scales_b_stride, kb_begin));
     constexpr int kRowsOfB = (BN + 31) / 32;
     uint32_t slot = 0, slot_phase = 0;
     bool ok = true;
     for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
       int ta, tb;
       raster(t, p.tiles_a, p.tiles_b, ta, tb);
-      const uint8_t* row_a[4];
-      const uint8_t* row_b[kRowsOfB];
+      const uint8_t* row[4 + kRowsOfB];  // of A, then of B
 #pragma unroll
-      for (int c = 0; c < 4; ++c) row_a[c] = p.scales_a + min((PAIR ? ta * 2 + rank : ta) * kRowsA + c * 32 + lane, p.rows_a - 1) * p.scales_a_stride;
+      for (int c = 0; c < 4; ++c) row[c] = p.scales_a + min((PAIR ? ta * 2 + rank : ta) * kRowsA + c * 32 + lane, p.rows_a - 1) * p.scales_a_stride;
 #pragma unroll
-      for (int c = 0; c < kRowsOfB; ++c) row_b[c] = p.scales_b + min(tb * BN + c * 32 + lane, p.rows_b - 1) * p.scales_b_stride;
+      for (int c = 0; c < kRowsOfB; ++c) row[4 + c] = p.scales_b + min(tb * BN + c * 32 + lane, p.rows_b - 1) * p.scales_b_stride;
       for (int kb = kb_begin; kb < kb_end; kb += 4 * kSlotWords) {
-        uint32_t a[4][4], b[kRowsOfB][4];  // [32 rows each][word]
-        load_scales<4>(a, row_a, kb, p.k_blocks, align_a);
-        load_scales<kRowsOfB>(b, row_b, kb, p.k_blocks, align_b);
+        uint32_t w[4 + kRowsOfB][4];  // [32 rows each][word]
+        load_scales<4 + kRowsOfB>(w, row, kb, p.k_blocks, align);
         if (!wait_warp<false>(smem_u32(&scale_empty[slot]), slot_phase ^ 1, abort_flag)) {
           if (!*abort_flag && lane == 0) record(p.status, 1, blockIdx.x, t, 600 + slot);
           *abort_flag = 1;
@@ -468,13 +526,12 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
         uint8_t* dst = scale_ring + slot * C::kScaleSlotBytes + lane * 16;
 #pragma unroll
         for (int i = 0; i < kSlotWords; ++i) {
-          *reinterpret_cast<uint4*>(dst + i * C::kWordBytes) = make_uint4(a[0][i], a[1][i], a[2][i], a[3][i]);
 #pragma unroll
-          for (int c = 0; c < kRowsOfB; c += 4) {
-            uint32_t w[4];
+          for (int c = 0; c < 4 + kRowsOfB; c += 4) {
+            uint32_t v[4];  // columns past B's last rows: any
 #pragma unroll
-            for (int j = 0; j < 4; ++j) w[j] = c + j < kRowsOfB ? b[c + j < kRowsOfB ? c + j : 0][i] : 0x7F7F7F7Fu;
-            *reinterpret_cast<uint4*>(dst + i * C::kWordBytes + 512 * (1 + c / 4)) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 4; ++j) v[j] = w[c + j < 4 + kRowsOfB ? c + j : 0][i];
+            *reinterpret_cast<uint4*>(dst + i * C::kWordBytes + 128 * c) = make_uint4(v[0], v[1], v[2], v[3]);
           }
         }
         fence_proxy_async_smem();
@@ -513,26 +570,22 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
         // time; sharing the tile, it leaves its partial sums in the operand ring, which is free: the
         // last MMA has read it.
         const int tokens = min(BN, p.rows_b - tb * BN);
-        float* partial = reinterpret_cast<float*>(smem);
+        float* partial = reinterpret_cast<float*>(smem) + q * 32 + lane;
         const int col = row0 + lane;
+        const int64_t stride = p.out_stride * (p.out_f32 ? 4 : 2);
+        char* dst = static_cast<char*>(p.out) + tb * BN * stride + static_cast<int64_t>(col) * (p.out_f32 ? 4 : 2);
 #pragma unroll 1
-        for (int c = 0; c < BN; c += 16) {
-          if (c >= tokens) break;
+        for (int c = 0; c < tokens; c += 16) {
           uint32_t v[16];
           tmem_ld_32x32b_x16(t_row + c, v);
           tmem_ld_wait();
           if (p.split > 1) {
 #pragma unroll
-            for (int j = 0; j < 16; ++j) partial[(c + j) * kReducePitch + q * 32 + lane] = __uint_as_float(v[j]);
+            for (int j = 0; j < 16; ++j) partial[(c + j) * kReducePitch] = __uint_as_float(v[j]);
           } else if (col < p.rows_a) {
-            const int64_t at = static_cast<int64_t>(tb * BN + c) * p.out_stride + col;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              if (c + j < tokens) {
-                if (p.out_f32) static_cast<float*>(p.out)[at + j * p.out_stride] = __uint_as_float(v[j]);
-                else static_cast<__nv_bfloat16*>(p.out)[at + j * p.out_stride] = __float2bfloat16_rn(__uint_as_float(v[j]));
-              }
-            }
+            if (p.out_f32) store_tokens<float>(dst, stride, v, tokens - c);
+            else store_tokens<__nv_bfloat16>(dst, stride, v, tokens - c);
+            dst += 16 * stride;
           }
         }
         tcgen05_fence_before();
@@ -614,28 +667,10 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
     const int tokens = min(BN, p.rows_b - tb * BN);
     const int pieces = tokens * (kRowsA / 4);
     if (!*abort_flag) {
-      for (int i = rank * kThreads + static_cast<int>(threadIdx.x); i < pieces; i += p.split * kThreads) {
-        const int token = i / (kRowsA / 4), c4 = (i % (kRowsA / 4)) * 4;
-        const uint32_t at = smem_u32(smem) + (token * kReducePitch + c4) * 4;
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int s = 0; s < p.split; ++s) {
-          const float4 v = ld_cluster_f32x4(at, s);
-          sum.x += v.x;
-          sum.y += v.y;
-          sum.z += v.z;
-          sum.w += v.w;
-        }
-        const float e[4] = {sum.x, sum.y, sum.z, sum.w};
-        const int col = ta * kRowsA + c4;
-        const int64_t dst = static_cast<int64_t>(tb * BN + token) * p.out_stride + col;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          if (col + j < p.rows_a) {
-            if (p.out_f32) static_cast<float*>(p.out)[dst + j] = e[j];
-            else static_cast<__nv_bfloat16*>(p.out)[dst + j] = __float2bfloat16_rn(e[j]);
-          }
-        }
-      }
+      const uint32_t base = smem_u32(smem);
+      if (p.split <= 2) reduce_pieces<2, 4>(p, base, rank, ta * kRowsA, tb * BN, pieces);
+      else if (p.split <= 4) reduce_pieces<4, 2>(p, base, rank, ta * kRowsA, tb * BN, pieces);
+      else reduce_pieces<8, 1>(p, base, rank, ta * kRowsA, tb * BN, pieces);
     }
     __syncwarp();
     cluster_sync();  // no block leaves while another reads its shared memory
@@ -719,44 +754,56 @@ int32_t encode_operand(CUtensorMap* map, const void* base, int64_t rows, int64_t
   return cake::encode_tensor_map_as(map, base, 2, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_DATA_TYPE_UINT8);
 }
 
-// What a call runs: the tile, and for few tokens the blocks that share one.
+// What a call runs: the tile, and for narrow tiles the blocks that share one.
 struct Choice {
   int tile, split;
 };
 
-bool is_narrow(int tile) { return tile <= 64; }
+bool is_narrow(int tile) { return tile <= 128; }
+
+// Nanoseconds that a call of this shape is expected to take, from times measured at 1 to 1024 rows and
+// extents of 1024 to 8192 (graph replays, one after the other): good to about a fifth, and the neighbours of the
+// least are within that of each other. Some 4000 pass before the first and after the last k block.
+double narrow_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int split, int sm_count) {
+  const double blocks = static_cast<double>((n + 127) / 128) * ((m + tile - 1) / tile) * split;
+  const double kb = static_cast<double>((k_blocks + split - 1) / split);
+  // One k block of one block's: what the tensor core takes for 128 x 64 or less, more with the bytes that the
+  // SM has to fetch for it (and for the block it shares the SM with).
+  const bool alone = blocks <= sm_count;
+  const double k_block = tile <= 32 ? (alone ? 210 : 235) : tile == 64 ? (alone ? 245 : 330) : (alone ? 345 : 430);
+  const double waves = std::ceil(blocks / (2.0 * sm_count));
+  const double fetch = blocks * kb * (16384 + 128.0 * tile) / 17000;
+  // HBM at 5.0 TB/s with one block's ring in flight per SM, 6.2 with two; less if several blocks want the same rows.
+  const double hbm = static_cast<double>(n) * k_blocks * 128 / (alone ? 5000 : 6200) * (m > tile ? 1.25 : 1);
+  const double sharing = split > 1 ? waves * split * (200 + 6.0 * tile) : 0;
+  return 4000 + 10.0 * tile + (waves - 1) * 2000 + std::max({waves * kb * k_block, fetch, hbm}) + sharing;
+}
+
+double wide_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int sm_count) {
+  const double tiles = static_cast<double>((m + 255) / 256) * ((n + tile - 1) / tile), pairs = sm_count / 2;
+  const double waves = std::ceil(tiles / pairs);
+  const double k_block = (60 + 1.07 * tile) * (tiles > 0.6 * pairs ? 1.18 : 1);  // L2 is shared by as many
+  // 256 columns leave no second accumulator, so nothing hides a tile's epilogue.
+  return 4500 + waves * k_blocks * k_block + (tile == 256 ? waves : 1) * 10 * tile;
+}
 
 Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count) {
-  Choice c = {d.tile, d.k_split};
+  Choice best = {d.tile, d.k_split};
   const int64_t k_blocks = (d.k + cake::kBlockK - 1) / cake::kBlockK;
-  if (c.tile == 0) {
-    if (m <= 16) c.tile = 16;
-    else if (m <= 32) c.tile = 32;
-    else if (m <= 256) c.tile = 64;
-    else {
-      int64_t best = 0;
-      const int64_t pairs = sm_count / 2;
-      for (int tile : {128, 192, 224, 256}) {
-        const int64_t tiles = ((m + 255) / 256) * ((d.n + tile - 1) / tile);
-        const int64_t waves = (tiles + pairs - 1) / pairs;
-        // Cycles: a k block takes 2 tile, but not less than 400; an epilogue that nothing hides 16 a column.
-        const int64_t k_block = 2 * tile > 400 ? 2 * tile : 400;
-        const int64_t cost = waves * k_blocks * k_block + (tile == 256 ? waves : 1) * 16 * tile;
-        if (best == 0 || cost <= best) {
-          best = cost;
-          c.tile = tile;
-        }
+  double least = 0;
+  for (int tile : {16, 32, 64, 128, 192, 224, 256}) {
+    if (d.tile != 0 && tile != d.tile) continue;
+    for (int split : {1, 2, 4, 8}) {
+      if (split > 1 && (!is_narrow(tile) || split > k_blocks || (d.k_split != 0 && d.tile != 0))) break;
+      const double ns = is_narrow(tile) ? narrow_ns(m, d.n, k_blocks, tile, split, sm_count) : wide_ns(m, d.n, k_blocks, tile, sm_count);
+      if (least == 0 || ns < least) {
+        least = ns;
+        best = {tile, split};
       }
     }
   }
-  if (!is_narrow(c.tile)) c.split = 1;
-  else if (c.split == 0) {
-    const int64_t tiles = ((d.n + 127) / 128) * ((m + c.tile - 1) / c.tile);
-    c.split = 1;
-    while (c.split < 8 && 2 * c.split * tiles <= sm_count && 2 * c.split <= k_blocks) c.split *= 2;
-  }
-  if (c.split > k_blocks) c.split = static_cast<int>(k_blocks);
-  return c;
+  if (d.k_split > 0) best.split = static_cast<int>(std::min<int64_t>(d.k_split, k_blocks));
+  return best;
 }
 
 }  // namespace
@@ -777,7 +824,7 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
   if (d.tile != 0 && d.tile != 16 && d.tile != 32 && d.tile != 64 && d.tile != 128 && d.tile != 192 && d.tile != 224 && d.tile != 256)
     return fail(CAKE_ERR_UNSUPPORTED, "tile must be 0, 16, 32, 64, 128, 192, 224 or 256, got %d", d.tile);
   if (d.k_split < 0 || d.k_split > 8 || (d.k_split > 1 && (!is_narrow(d.tile) || d.tile == 0)))
-    return fail(CAKE_ERR_INVALID_ARGUMENT, "k_split must be 0 to 8, and above 1 only with tile 16, 32 or 64, got %d", d.k_split);
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "k_split must be 0 to 8, and above 1 only with tile 16, 32, 64 or 128, got %d", d.k_split);
   if (m < 0 || m > INT32_MAX / 2) return fail(CAKE_ERR_INVALID_ARGUMENT, "m must be 0 to 2^30 - 1, got %lld", (long long)m);
   if (m == 0) return CAKE_OK;
   if (!lhs || !lhs_scales || !rhs || !rhs_scales || !out) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_enqueue: null argument");
@@ -852,7 +899,7 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
     case 16: return launch<16, true>(device, map_a, map_b, map_out, p, s);
     case 32: return launch<32, true>(device, map_a, map_b, map_out, p, s);
     case 64: return launch<64, true>(device, map_a, map_b, map_out, p, s);
-    case 128: return launch<128, false>(device, map_a, map_b, map_out, p, s);
+    case 128: return launch<128, true>(device, map_a, map_b, map_out, p, s);
     case 192: return launch<192, false>(device, map_a, map_b, map_out, p, s);
     case 224: return launch<224, false>(device, map_a, map_b, map_out, p, s);
     default: return launch<256, false>(device, map_a, map_b, map_out, p, s);

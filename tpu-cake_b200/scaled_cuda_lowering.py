@@ -245,9 +245,9 @@ class CudaRmsNormQuantizePlan:
 @dataclass(frozen=True)
 class CudaScaledMatmulPlan:
     """out [m, n] = lhs [m, k] rhs [n, k]^T over dequantised operands, accumulated in f32 and rounded once
-    to ``output_dtype``. ``tile`` and ``k_split`` override the library's choice (0): tiles of 16, 32 or 64
-    tokens by 128 columns with 1 to 8 blocks sharing a tile's contraction, or of 256 tokens by 128,
-    192, 224 or 256 columns. Runs on one mesh position."""
+    to ``output_dtype``. ``tile`` and ``k_split`` override the library's choice (0): tiles of 16, 32, 64 or
+    128 tokens by 128 columns with 1 to 8 blocks sharing a tile's contraction, or of 256 tokens by 192,
+    224 or 256 columns. Runs on one mesh position."""
 
     name: str
     n: int
@@ -263,8 +263,8 @@ class CudaScaledMatmulPlan:
             raise ValueError(f"output dtype must be f32 or bf16, got {self.output_dtype}")
         if self.tile not in (0, 16, 32, 64, 128, 192, 224, 256):
             raise ValueError(f"tile must be 0, 16, 32, 64, 128, 192, 224 or 256, got {self.tile}")
-        if not 0 <= self.k_split <= 8 or (self.k_split > 1 and self.tile not in (16, 32, 64)):
-            raise ValueError(f"k_split must be 0 to 8, and above 1 only with tile 16, 32 or 64, got {self.k_split}")
+        if not 0 <= self.k_split <= 8 or (self.k_split > 1 and self.tile not in (16, 32, 64, 128)):
+            raise ValueError(f"k_split must be 0 to 8, and above 1 only with tile 16, 32, 64 or 128, got {self.k_split}")
 
     def render_executable_source(self) -> str:
         return _source("block-scaled matmul", "cake_scaled_matmul_sm100", self, ("n", "k", "output_dtype", "tile", "k_split"))
