@@ -779,15 +779,18 @@ double narrow_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int split, in
   return 4000 + 10.0 * tile + (waves - 1) * 2000 + std::max({waves * kb * k_block, fetch, hbm}) + sharing;
 }
 
-double wide_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int sm_count) {
+// tensor_store: the output's rows are whole 16-byte pieces. Other rows leave 64 bytes at a time, most of them
+// parts of 32-byte sectors: four times as slow (1001 x 5120 x 4096: 21 us, x 4099: 29 us).
+double wide_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int sm_count, bool tensor_store) {
   const double tiles = static_cast<double>((m + 255) / 256) * ((n + tile - 1) / tile), pairs = sm_count / 2;
   const double waves = std::ceil(tiles / pairs);
-  const double k_block = (60 + 1.07 * tile) * (tiles > 0.6 * pairs ? 1.18 : 1);  // L2 is shared by as many
+  const double main_loop = k_blocks * (60 + 1.07 * tile) * (tiles > 0.6 * pairs ? 1.18 : 1);  // L2 is shared by as many
+  const double epilogue = tile * (tensor_store ? 10 : 38);
   // 256 columns leave no second accumulator, so nothing hides a tile's epilogue.
-  return 4500 + waves * k_blocks * k_block + (tile == 256 ? waves : 1) * 10 * tile;
+  return 4500 + (tile == 256 ? waves * (main_loop + epilogue) : waves * std::max(main_loop, epilogue) + epilogue);
 }
 
-Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count) {
+Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count, bool tensor_store) {
   Choice best = {d.tile, d.k_split};
   const int64_t k_blocks = (d.k + cake::kBlockK - 1) / cake::kBlockK;
   double least = 0;
@@ -795,7 +798,7 @@ Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count) {
     if (d.tile != 0 && tile != d.tile) continue;
     for (int split : {1, 2, 4, 8}) {
       if (split > 1 && (!is_narrow(tile) || split > k_blocks || (d.k_split != 0 && d.tile != 0))) break;
-      const double ns = is_narrow(tile) ? narrow_ns(m, d.n, k_blocks, tile, split, sm_count) : wide_ns(m, d.n, k_blocks, tile, sm_count);
+      const double ns = is_narrow(tile) ? narrow_ns(m, d.n, k_blocks, tile, split, sm_count) : wide_ns(m, d.n, k_blocks, tile, sm_count, tensor_store);
       if (least == 0 || ns < least) {
         least = ns;
         best = {tile, split};
@@ -852,7 +855,10 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
   Device device;
   int32_t rc = current_device(&device);
   if (rc) return rc;
-  const Choice c = choose(d, m, device.sm_count);
+  // Tensor stores write whole 16-byte pieces, also where the row ends inside one: only rows of whole pieces
+  // leave what lies behind them alone.
+  const bool tensor_store = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && out_row_stride * osize % 16 == 0 && d.n * osize % 16 == 0;
+  const Choice c = choose(d, m, device.sm_count, tensor_store);
   const bool narrow = is_narrow(c.tile);
   cake::Params p;
   memset(&p, 0, sizeof(p));
@@ -876,9 +882,7 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
   p.out = out;
   p.out_stride = out_row_stride;
   p.status = status_device;
-  // Tensor stores write whole 16-byte pieces, also where the row ends inside one: only rows of whole pieces
-  // leave what lies behind them alone.
-  p.tma_store = !narrow && (reinterpret_cast<uintptr_t>(out) & 15) == 0 && out_row_stride * osize % 16 == 0 && d.n * osize % 16 == 0;
+  p.tma_store = !narrow && tensor_store;
 
   CUtensorMap map_a, map_b, map_out;
   memset(&map_out, 0, sizeof(map_out));
