@@ -382,3 +382,30 @@ def test_entry_points_refuse_what_tensor_maps_cannot_hold(cuda_device):
         plan.invoke(executable, lhs, lhs_scales, bad_base, lhs_scales)
     with pytest.raises(ValueError, match="must be on"):
         plan.invoke(executable, lhs.cpu(), lhs_scales, lhs, lhs_scales)
+
+
+@pytest.mark.parametrize("rows", [3, 200])
+def test_mlp_plan_gives_what_its_calls_give(cuda_device, rows):
+    mlp = Mlp(cuda_device, 640, 1000)
+    x, residual = activations(1, rows, 640, "bf16", cuda_device), activations(2, rows, 640, "bf16", cuda_device)
+    plan = scaled.CudaScaledMlpPlan(name="layer", hidden=640, inner=1000)
+    executable = plan.build(cuda_device)
+    weights = plan.quantize_weights(executable, mlp.norm_weight, mlp.up, mlp.down)
+    out, summed = plan.invoke(executable, weights, x, residual)
+    want, want_residual = mlp(x, residual.clone())
+    assert executable.status() == (0, 0, 0, 0)
+    assert torch.equal(out, want) and torch.equal(summed, want_residual)
+    executable.close()
+
+
+def test_run_scaled_mlp_writes_a_bundle(cuda_device, tmp_path):
+    import json
+
+    from tpu_cake_b200 import cli
+
+    assert cli.main(["run-scaled-mlp", str(tmp_path / "out"), "--rows", "33", "--hidden", "520", "--inner", "776", "--measured-iterations", "3"]) == 0
+    result = json.loads((tmp_path / "out" / "result.json").read_text())
+    assert result["passed"] and result["median_ns"] > 0 and max(result["share_of_bound"].values()) <= 1
+    assert {a["role"] for a in result["artifacts"]} >= {"contract", "lowered_source", "correctness", "execution_ledger", "source_state"}
+    with pytest.raises(FileExistsError):
+        cli.main(["run-scaled-mlp", str(tmp_path / "out")])

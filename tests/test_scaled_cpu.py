@@ -226,3 +226,40 @@ def test_null_descriptor_is_an_error_and_no_rows_are_no_work():
     assert ctypes.sizeof(_native.ScaledMatmulDesc) == 32
     assert _native.load().cake_scaled_matmul_enqueue(None, 1, *[None, 0] * 5, None, None) == _native.CAKE_ERR_INVALID_ARGUMENT
     assert _matmul(m=0, lhs=None, lhs_scales=None, rhs=None, rhs_scales=None, out=None) == _native.CAKE_OK
+
+
+def test_mlp_plan_and_runner_refuse_bad_shapes(tmp_path):
+    from tpu_cake_b200 import cli, scaled_runner
+
+    plan = scaled.CudaScaledMlpPlan(name="layer", hidden=640, inner=1000)
+    assert plan.up.n == 2000 and plan.up.k == 640 and plan.down.n == 640 and plan.down.k == 1000 and plan.gate.gate == "silu"
+    for kernel in ("cake_rms_norm_quantize_sm100", "cake_scaled_matmul_sm100", "cake_quantize_rows_sm100"):
+        assert kernel in plan.render_executable_source()
+    for wrong in ({"hidden": scaled.MAX_NORM_COLUMNS + 1, "inner": 8}, {"hidden": 8, "inner": 0}):
+        with pytest.raises(ValueError):
+            scaled.CudaScaledMlpPlan(name="layer", **wrong)
+    with pytest.raises(ValueError, match="up must be"):
+        plan.quantize_weights(None, None, torch.zeros(4, 4), torch.zeros(4, 4))
+    with pytest.raises(ValueError, match="positive"):
+        scaled_runner.run_scaled_mlp(tmp_path / "out", rows=0, hidden=64, inner=64)
+    if not torch.cuda.is_available():
+        with pytest.raises(RuntimeError, match="no CPU fallback"):
+            cli.main(["run-scaled-mlp", str(tmp_path / "out")])
+    assert not (tmp_path / "out").exists()
+
+
+def test_runner_bounds_reject_a_wrong_scale():
+    from tpu_cake_b200 import scaled_runner
+
+    v = torch.randn(4, 300, generator=torch.Generator().manual_seed(0)).double()
+    codes, scales = oracle.quantize(v.numpy())
+    codes = torch.from_numpy(codes).float().to(torch.float8_e4m3fn)
+    byte = torch.from_numpy(np.log2(scales) + 127).to(torch.uint8)
+    assert scaled_runner._check_codes(codes, byte.view(torch.float8_e8m0fnu), v) <= 1
+    byte[2, 1] += 1
+    assert scaled_runner._check_codes(codes, byte.view(torch.float8_e8m0fnu), v) > 1
+    lhs, rhs = v, torch.randn(7, 300, generator=torch.Generator().manual_seed(1)).double()
+    out = (lhs @ rhs.t()).to(torch.bfloat16)
+    assert scaled_runner._check_matmul(out, lhs, rhs) <= 1
+    out[1, 2] *= 1.02
+    assert scaled_runner._check_matmul(out, lhs, rhs) > 1

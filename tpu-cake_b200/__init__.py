@@ -11,5 +11,6 @@ __all__ = [
     "workloads",
     "cuda_lowering",
     "rpa_cuda_lowering",
+    "scaled_cuda_lowering",
     "mesh",
 ]

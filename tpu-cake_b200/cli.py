@@ -2,7 +2,8 @@
 (src/tpu_cake/cli.py:154-425): ``run-matmul`` (:216-232), ``search-matmul``, ``render-workload`` and
 ``verify-schedule`` for the distributed matmul, ``estimate`` for its cost model, ``experiment``
 (:150,212,667-676) for the experiment records of the matmul and the two Inkling RPA workloads,
-``run-rpa`` (the device entry point, src/tpu_cake/rpa_device_main.py), ``inspect-profile``
+``run-rpa`` (the device entry point, src/tpu_cake/rpa_device_main.py), ``run-scaled-mlp`` (this backend's 8-bit
+MLP layer), ``inspect-profile``
 (:187,572-601: exit code 1 when the capture is rejected) and the receipt commands.
 
     python -m torch.distributed.run --nproc-per-node 8 __graft_entry__.py cli run-matmul OUT \
@@ -55,6 +56,13 @@ def main(argv: list[str] | None = None) -> int:
     run_rpa.add_argument("--kv-chunk-tokens", type=int, default=0)
     run_rpa.add_argument("--from-physical", type=Path, metavar="PHYSICAL.XDSL",
                          help="run the kernel a saved physical schedule holds instead of this backend's own schedule of the experiment")
+    scaled = commands.add_parser("run-scaled-mlp", help="run the 8-bit gated MLP layer (norm, projections and gate on e4m3 operands) and write a run bundle")
+    scaled.add_argument("output_dir", type=Path)
+    scaled.add_argument("--rows", type=int, default=64)
+    scaled.add_argument("--hidden", type=int, default=1024)
+    scaled.add_argument("--inner", type=int, default=2048)
+    scaled.add_argument("--warmup-iterations", type=int, default=3)
+    scaled.add_argument("--measured-iterations", type=int, default=10)
     surface = commands.add_parser("run-rpa-surface", help="run the 2 x 4 sharded RPA surface protocol (five seeds, two executions each, exact repeats and cache; chained timing rounds)")
     surface.add_argument("output_dir", type=Path)
     surface.add_argument("--emulate-on-one-gpu", action="store_true", help="run the eight mesh positions one after the other on this GPU (they exchange nothing); recorded as emulated")
@@ -111,6 +119,13 @@ def main(argv: list[str] | None = None) -> int:
 
         saved = [] if args.from_physical is None else ["--from-physical", str(args.from_physical)]
         return rpa_runner.rpa_device_main([str(args.output_dir), "--mode", args.mode, "--kv-chunk-tokens", str(args.kv_chunk_tokens), *saved])
+    if args.command == "run-scaled-mlp":
+        from . import scaled_runner
+
+        result = scaled_runner.run_scaled_mlp(args.output_dir, rows=args.rows, hidden=args.hidden, inner=args.inner,
+                                              warmup_iterations=args.warmup_iterations, measured_iterations=args.measured_iterations)
+        print(f"SCALED_MLP_PASSED run_id={result['run_id'][:12]} median_ns={result['median_ns']:.0f} worst_share_of_bound={max(result['share_of_bound'].values()):.3f}")
+        return 0
     if args.command == "run-rpa-surface":
         from . import rpa_surface_runner
         from .mesh import ProcessMesh

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes
 from dataclasses import dataclass
+from functools import cached_property
 
 import torch
 
@@ -289,3 +290,87 @@ class CudaScaledMatmulPlan:
         executable.enqueue(m, lhs.data_ptr(), lhs_stride, lhs_scales.data_ptr(), lhs_scales_stride, rhs.data_ptr(), rhs_stride,
                            rhs_scales.data_ptr(), rhs_scales_stride, out.data_ptr(), out_stride)
         return out
+
+
+@dataclass(frozen=True)
+class ScaledMlpWeights:
+    """A layer's parameters as the kernels take them: the norm's vector and the two projections as (codes, scales)."""
+
+    norm: torch.Tensor
+    up: tuple[torch.Tensor, torch.Tensor]    # [2 * inner, hidden]: gate rows, then up rows
+    down: tuple[torch.Tensor, torch.Tensor]  # [hidden, inner]
+
+
+class ScaledMlpExecutable:
+    """The executables of a layer's four calls on one GPU."""
+
+    def __init__(self, plan: "CudaScaledMlpPlan", device: torch.device):
+        self.rows = plan.norm.build(device)
+        self.up = plan.up.build(device)
+        self.down = plan.down.build(device)
+        self.device = self.rows.device
+
+    def status(self) -> tuple[int, int, int, int]:
+        """Raises if a matmul's bounded wait ran out."""
+        self.up.status()
+        return self.down.status()
+
+    def close(self) -> None:
+        """Nothing to release: here for the executables' common surface."""
+
+
+@dataclass(frozen=True)
+class CudaScaledMlpPlan:
+    """The 8-bit gated MLP of a decoder layer, four calls: residual addition, norm and quantisation; the gate
+    and up projection; silu(gate) * up and quantisation; the down projection."""
+
+    name: str
+    hidden: int
+    inner: int
+    epsilon: float = 1e-5
+
+    def __post_init__(self) -> None:
+        self.norm, self.up, self.gate, self.down  # their own checks
+
+    @cached_property
+    def norm(self) -> CudaRmsNormQuantizePlan:
+        return CudaRmsNormQuantizePlan(name=f"{self.name}-norm", columns=self.hidden, epsilon=self.epsilon)
+
+    @cached_property
+    def up(self) -> CudaScaledMatmulPlan:
+        return CudaScaledMatmulPlan(name=f"{self.name}-up", n=2 * self.inner, k=self.hidden)
+
+    @cached_property
+    def gate(self) -> CudaQuantizeRowsPlan:
+        return CudaQuantizeRowsPlan(name=f"{self.name}-gate", columns=self.inner, gate="silu")
+
+    @cached_property
+    def down(self) -> CudaScaledMatmulPlan:
+        return CudaScaledMatmulPlan(name=f"{self.name}-down", n=self.hidden, k=self.inner)
+
+    def render_executable_source(self) -> str:
+        return "".join(plan.render_executable_source() for plan in (self.norm, self.up, self.gate, self.down))
+
+    def source_sha256(self) -> str:
+        return text_sha256(self.render_executable_source())
+
+    def build(self, device: torch.device | None = None) -> ScaledMlpExecutable:
+        return ScaledMlpExecutable(self, _device(device))
+
+    def quantize_weights(self, executable: ScaledMlpExecutable, norm, up, down) -> ScaledMlpWeights:
+        """bf16 parameters to what ``invoke`` takes, once when a model is loaded: ``up`` [2 * inner, hidden] is
+        the gate projection's rows followed by the up projection's, ``down`` [hidden, inner]."""
+        if not isinstance(up, torch.Tensor) or not isinstance(down, torch.Tensor) or up.shape != (2 * self.inner, self.hidden) \
+                or down.shape != (self.hidden, self.inner):
+            raise ValueError(f"up must be [{2 * self.inner}, {self.hidden}] and down [{self.hidden}, {self.inner}]")
+        return ScaledMlpWeights(
+            norm=norm,
+            up=CudaQuantizeRowsPlan(name=f"{self.name}-up-weights", columns=self.hidden).invoke(executable.rows, up),
+            down=CudaQuantizeRowsPlan(name=f"{self.name}-down-weights", columns=self.inner).invoke(executable.rows, down),
+        )
+
+    def invoke(self, executable: ScaledMlpExecutable, weights: ScaledMlpWeights, x, residual, *, out=None, residual_out=None):
+        """(layer output bf16 [rows, hidden], x + residual): bf16 ``x`` and ``residual`` [rows, hidden]."""
+        codes, scales, summed = self.norm.invoke(executable.rows, x, weights.norm, residual, residual_out=residual_out)
+        projected = self.up.invoke(executable.up, codes, scales, *weights.up)
+        return self.down.invoke(executable.down, *self.gate.invoke(executable.rows, projected), *weights.down, out=out), summed
