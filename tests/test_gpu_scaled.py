@@ -409,3 +409,99 @@ def test_run_scaled_mlp_writes_a_bundle(cuda_device, tmp_path):
     assert {a["role"] for a in result["artifacts"]} >= {"contract", "lowered_source", "correctness", "execution_ledger", "source_state"}
     with pytest.raises(FileExistsError):
         cli.main(["run-scaled-mlp", str(tmp_path / "out")])
+
+
+# ------------------------------------------------------------------------------------------ far apart, first calls
+
+
+def test_rows_more_than_32_bits_apart(cuda_device):
+    """Row strides of 2^31 + 8 elements: the third row starts beyond 2^32 elements (8 GiB)."""
+    stride = (1 << 31) + 8
+    held = torch.empty(2 * stride + 512, dtype=torch.bfloat16, device=cuda_device)
+    x = held.as_strided((3, 512), (stride, 1))
+    x.copy_(activations(1, 3, 512, "bf16", cuda_device))
+    expected = oracle.quantize(numpy64(x))
+    plan = scaled.CudaQuantizeRowsPlan(name="t", columns=512)
+    codes, scales = plan.invoke(plan.build(cuda_device), x)
+    assert np.array_equal(numpy64(codes), expected[0]) and np.array_equal(scale_values(scales), expected[1])
+    norm = scaled.CudaRmsNormQuantizePlan(name="t", columns=512)
+    residual = activations(2, 3, 512, "bf16", cuda_device)
+    summed = (x.float() + residual.float()).to(torch.bfloat16)
+    want, _h = oracle.rms_norm(numpy64(x), np.ones(512), 1e-5, numpy64(residual))
+    codes, scales, _ = norm.invoke(norm.build(cuda_device), x, torch.ones(512, dtype=torch.bfloat16, device=cuda_device), residual, residual_out=x)
+    check_close(codes, scales, want, NORM_DELTA)
+    assert torch.equal(x, summed)
+
+
+@pytest.mark.parametrize("m, n, k, tile", [(40000, 65540, 130, 0), (40000, 65540, 130, 128), (40000, 65539, 130, 224)])
+def test_matmul_outputs_beyond_32_bits(cuda_device, m, n, k, tile):
+    """2.6 billion outputs: checked where the last rows and columns lie."""
+    lhs, lhs_scales = operand(1, m, k, cuda_device, exact=True)
+    rhs, rhs_scales = operand(2, n, k, cuda_device, exact=True)
+    plan = scaled.CudaScaledMatmulPlan(name="t", n=n, k=k, tile=tile)
+    executable = plan.build(cuda_device)
+    out = plan.invoke(executable, lhs, lhs_scales, rhs, rhs_scales)
+    assert executable.status() == (0, 0, 0, 0)
+    for rows in (slice(0, 8), slice(32760, 32776), slice(m - 40, m)):
+        expected = oracle.matmul(numpy64(lhs[rows]), scale_values(lhs_scales[rows]), numpy64(rhs), scale_values(rhs_scales))
+        assert torch.equal(out[rows].cpu(), torch.from_numpy(expected).to(torch.bfloat16))
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import sys, torch
+sys.path.insert(0, {root!r})
+import __graft_entry__
+__graft_entry__.load_package()
+from tpu_cake_b200 import scaled_cuda_lowering as scaled
+device = torch.device("cuda", 0)
+x = torch.randn(300, 512, device=device).to(torch.bfloat16)
+w = torch.randn({n}, 512, device=device).to(torch.bfloat16)
+quantize = scaled.CudaQuantizeRowsPlan(name="t", columns=512)
+matmul = scaled.CudaScaledMatmulPlan(name="t", n={n}, k=512)
+rows, product = quantize.build(device), matmul.build(device)
+def layer():
+    return matmul.invoke(product, *quantize.invoke(rows, x), *quantize.invoke(rows, w))
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = layer()
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, layer()) and product.status() == (0, 0, 0, 0)
+x.mul_(2)
+graph.replay()
+torch.cuda.synchronize()
+assert torch.equal(out, layer())
+"""
+
+
+@pytest.mark.parametrize("n", [64, 20000])
+def test_the_first_call_of_a_process_may_be_captured(cuda_device, n):
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = str(Path(__file__).resolve().parent.parent)
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE.format(root=root, n=n)], capture_output=True, text=True, timeout=180, check=False)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
+def test_calls_on_two_streams_overlap(cuda_device):
+    """Wide and narrow matmuls and row kernels of two streams at once, many times: no call sees another."""
+    streams = [torch.cuda.Stream(cuda_device) for _ in range(3)]
+    work = []
+    for i, (m, n, k) in enumerate(((300, 2048, 1024), (5, 4096, 2048), (70, 1000, 1500))):
+        x = activations(i, m, k, "bf16", cuda_device)
+        w = activations(10 + i, n, k, "bf16", cuda_device)
+        quantize, matmul = scaled.CudaQuantizeRowsPlan(name="t", columns=k), scaled.CudaScaledMatmulPlan(name="t", n=n, k=k, output_dtype="f32")
+        rows, product = quantize.build(cuda_device), matmul.build(cuda_device)
+        weights = quantize.invoke(rows, w)
+        work.append((matmul, product, quantize, rows, x, weights, matmul.invoke(product, *quantize.invoke(rows, x), *weights)))
+    torch.cuda.synchronize(cuda_device)
+    results = [[] for _ in work]
+    for _ in range(20):
+        for stream, (matmul, product, quantize, rows, x, weights, _want), got in zip(streams, work, results, strict=True):
+            with torch.cuda.stream(stream):
+                got.append(matmul.invoke(product, *quantize.invoke(rows, x), *weights))
+    torch.cuda.synchronize(cuda_device)
+    for (_m, product, _q, _r, _x, _w, want), got in zip(work, results, strict=True):
+        assert product.status() == (0, 0, 0, 0) and all(torch.equal(g, want) for g in got)

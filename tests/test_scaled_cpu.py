@@ -117,6 +117,10 @@ def test_invoke_refuses_wrong_operands():
         plain.invoke(recorder, x, weight, residual_out=x)
 
     matmul = scaled.CudaScaledMatmulPlan(name="p", n=32, k=256)
+    recorder.plan = scaled.CudaScaledMatmulPlan(name="p", n=32, k=512)
+    with pytest.raises(ValueError, match="another plan"):
+        matmul.invoke(recorder, None, None, None, None)
+    recorder.plan = scaled.CudaScaledMatmulPlan(name="p", n=32, k=256)
     codes, scales = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.ones(4, 2).to(torch.float8_e8m0fnu)
     rhs, rhs_scales = torch.zeros(32, 256).to(torch.float8_e4m3fn), torch.ones(32, 2).to(torch.float8_e8m0fnu)
     for wrong in ((codes[:, :255], scales, rhs, rhs_scales), (codes, scales[:3], rhs, rhs_scales), (codes, scales, rhs[:31], rhs_scales[:31]),
@@ -139,6 +143,8 @@ def _quantize(**overrides):
 @pytest.mark.parametrize("overrides, code, fragment", [
     ({"cols": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "columns"),
     ({"cols": 1 << 40}, _native.CAKE_ERR_INVALID_ARGUMENT, "columns"),
+    ({"rows": 1 << 30, "cols": 129, "x_stride": 129, "q_stride": 129, "scales_stride": 2}, _native.CAKE_ERR_UNSUPPORTED, "below 2^31"),
+    ({"x_stride": 1 << 32}, _native.CAKE_ERR_UNSUPPORTED, "below 2^32"),
     ({"rows": -1}, _native.CAKE_ERR_INVALID_ARGUMENT, "rows"),
     ({"rows": 1 << 31}, _native.CAKE_ERR_INVALID_ARGUMENT, "rows"),
     ({"dtype": 7}, _native.CAKE_ERR_INVALID_ARGUMENT, "dtype"),

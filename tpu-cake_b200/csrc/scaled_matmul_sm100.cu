@@ -8,17 +8,28 @@
 // With scales of any mantissa every 128-deep block's 128 x N products would have to be read back, scaled
 // and added in registers.
 //
-// One kernel template, two shapes of work. "A" is the 128-row operand of an MMA, "B" the one of BN rows.
-//   wide    A = lhs, B = rhs: 128 x BN output tiles, persistent blocks, two accumulators, so that a
-//           tile's epilogue runs under the next one's main loop.
+// One kernel template, two shapes of work. "A" is the 128-row operand of a block, "B" the one of BN rows.
+//   wide    A = lhs, B = rhs: 256 x BN output tiles by pairs of blocks (cta_group::2: each block loads 128 rows of
+//           A and half of B's, and one of them issues for both), persistent, with two accumulators, so that a
+//           tile's epilogue runs under the next one's main loop (one at BN = 256, where scales leave no
+//           room: for a single wave of tiles). A block fetches 128 + BN / 2 rows of 128 bytes for 2 BN cycles of
+//           MMA: 67 bytes a cycle at BN = 224; the 128 x 224 tile of a block alone needs 98, and L2 gives
+//           an SM about 64.
 //   narrow  A = rhs, B = lhs: 128 columns of the output by BN tokens. Few tokens: bound by reading rhs
-//           once, so BN is as small as the tokens allow, and the contraction of a tile is split over the
-//           blocks of a cluster, which add their partial sums through distributed shared memory in rank
-//           order (no workspace, no atomics: the same bits every time).
+//           once, and the contraction of a tile is split over the blocks of a cluster, which add their
+//           partial sums through distributed shared memory in rank order (no workspace, no atomics: the
+//           same bits every time). Two blocks share an SM: 6.2 TB/s where one reaches 5.0.
 // Warps: 0 TMA producer (128-byte swizzled rows of 128 codes, one k block per stage), 1 MMA issue and
-// tensor memory, 2 scales to shared memory, 3 scales on to tensor memory, 4-7 epilogue. Warp 2 gathers a 32-bit word -- four k blocks' bytes --
-// per operand row, so that scales are taken as they lie, with any stride, and puts them into shared memory
-// in the order tcgen05.cp wants: lane i's 16 bytes are rows i, 32 + i, 64 + i, 96 + i.
+// tensor memory, 2 scales to shared memory, 3 scales on to tensor memory, 4-7 epilogue. Warp 2 gathers a
+// 32-bit word -- four k blocks' bytes -- per operand row, so that scales are taken as they lie, with any
+// stride, and puts them into shared memory in the order tcgen05.cp wants: lane i's 16 bytes are rows i,
+// 32 + i, 64 + i, 96 + i.
+//
+// Measured (codes of normal values; device time of graph replays): 4096 x 8192 x 8192 182 us, 3.03 PFLOP/s, the
+// issuing warp taking 465 cycles per k block of 448 MMA cycles; 8192 x 16384 x 8192 840 us cold and 918 us
+// (2.40 PFLOP/s) after a second of load, when the power cap holds the clock near 1.26 GHz (cuBLAS in bf16:
+// 1.40 PFLOP/s then). Decode: 64 x 8192 x 16384 26.5 us (5.2 TB/s), 1 x 8192 x 8192 14.2 us: 4 us pass before the
+// first and after the last k block (dependency to first scales 1 to 1.5, cluster reduction 1.3).
 #include <cuda_bf16.h>
 #include <string.h>
 
@@ -110,13 +121,14 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, vol
 
 // The scale bytes of COUNT operand rows for 16 k blocks, from k block kb on, as four words each; anything past
 // the last k block. `align`: the rows' addresses and kb are multiples of it (16, 4 or 1). Every branch is the
-// whole warp's and has all rows' loads inside, so that they are under way together.
+// whole warp's and has all rows' loads inside, so that they are under way together. Ordinary loads: this kernel
+// may have started before the one that writes the scales ended, so they are not read-only for its lifetime.
 template <int COUNT>
 __device__ __forceinline__ void load_scales(uint32_t (&w)[COUNT][4], const uint8_t* const (&row)[COUNT], int kb, int k_blocks, int align) {
   if (align == 16 && kb + 16 <= k_blocks) {
 #pragma unroll
     for (int r = 0; r < COUNT; ++r) {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(row[r] + kb));
+      const uint4 v = *reinterpret_cast<const uint4*>(row[r] + kb);
       w[r][0] = v.x;
       w[r][1] = v.y;
       w[r][2] = v.z;
@@ -129,13 +141,13 @@ __device__ __forceinline__ void load_scales(uint32_t (&w)[COUNT][4], const uint8
     const int at = kb + 4 * i;
     if (align >= 4 && at + 4 <= k_blocks) {
 #pragma unroll
-      for (int r = 0; r < COUNT; ++r) w[r][i] = __ldg(reinterpret_cast<const uint32_t*>(row[r] + at));
+      for (int r = 0; r < COUNT; ++r) w[r][i] = *reinterpret_cast<const uint32_t*>(row[r] + at);
     } else if (at < k_blocks) {
       uint32_t byte[COUNT][4];
 #pragma unroll
       for (int r = 0; r < COUNT; ++r)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) byte[r][j] = __ldg(row[r] + min(at + j, k_blocks - 1));
+        for (int j = 0; j < 4; ++j) byte[r][j] = row[r][min(at + j, k_blocks - 1)];
 #pragma unroll
       for (int r = 0; r < COUNT; ++r) w[r][i] = byte[r][0] | (byte[r][1] << 8) | (byte[r][2] << 16) | (byte[r][3] << 24);
     } else {

@@ -103,13 +103,14 @@ class RowQuantizeExecutable(_Executable):
 
 
 class ScaledMatmulExecutable(_Executable):
-    """A matmul's descriptor and its status word on a GPU."""
+    """A matmul plan's descriptor and its status word on a GPU."""
 
-    def __init__(self, desc: _native.ScaledMatmulDesc, device: torch.device):
+    def __init__(self, plan: "CudaScaledMatmulPlan", desc: _native.ScaledMatmulDesc, device: torch.device):
         super().__init__(device)
+        self.plan = plan
         self._desc = desc
         self._desc_address = ctypes.addressof(desc)
-        self._status = torch.zeros(4, dtype=torch.int32, device=self.device)
+        self._status = torch.zeros(4, dtype=torch.int32).to(self.device)  # there when the copy returns, for any stream
         self._status_address = self._status.data_ptr()
 
     def enqueue(self, *arguments) -> None:
@@ -275,9 +276,11 @@ class CudaScaledMatmulPlan:
 
     def build(self, device: torch.device | None = None) -> ScaledMatmulExecutable:
         desc = _native.ScaledMatmulDesc(n=self.n, k=self.k, out_dtype=_CAKE_DTYPES[self.output_dtype], tile=self.tile, k_split=self.k_split)
-        return ScaledMatmulExecutable(desc, _device(device))
+        return ScaledMatmulExecutable(self, desc, _device(device))
 
     def invoke(self, executable: ScaledMatmulExecutable, lhs, lhs_scales, rhs, rhs_scales, *, out=None) -> torch.Tensor:
+        if executable.plan is not self and executable.plan != self:
+            raise ValueError(f"the executable was built from another plan: {executable.plan}")
         device, groups, dtype = executable.device, scale_columns(self.k), _DTYPES[self.output_dtype]
         m, lhs_stride = _rows(lhs, self.k, CODE_DTYPE, "lhs", device)
         _, lhs_scales_stride = _rows(lhs_scales, groups, SCALE_DTYPE, "lhs_scales", device, m)
