@@ -505,3 +505,37 @@ def test_calls_on_two_streams_overlap(cuda_device):
     torch.cuda.synchronize(cuda_device)
     for (_m, product, _q, _r, _x, _w, want), got in zip(work, results, strict=True):
         assert product.status() == (0, 0, 0, 0) and all(torch.equal(g, want) for g in got)
+
+
+def test_invoke_refuses_wrong_operands(cuda_device):
+    plan = scaled.CudaQuantizeRowsPlan(name="p", columns=100)
+    executable = plan.build(cuda_device)
+    x, weight = torch.zeros(4, 100, dtype=torch.bfloat16, device=cuda_device), torch.ones(100, dtype=torch.bfloat16, device=cuda_device)
+    for wrong in (x.float(), x[:, :99], x[0], x.t(), torch.zeros(4, 200, dtype=torch.bfloat16, device=cuda_device)[:, ::2], x[:1].expand(4, 100), None, x.cpu()):
+        with pytest.raises(ValueError, match="x must"):
+            plan.invoke(executable, wrong)
+    with pytest.raises(ValueError, match="codes must"):
+        plan.invoke(executable, x, codes=torch.zeros(3, 100, device=cuda_device).to(torch.float8_e4m3fn))
+    with pytest.raises(ValueError, match="scales must"):
+        plan.invoke(executable, x, scales=torch.ones(4, 2, device=cuda_device).to(torch.float8_e8m0fnu))
+    with pytest.raises(ValueError, match="x must"):
+        scaled.CudaQuantizeRowsPlan(name="p", columns=100, gate="silu").invoke(executable, x)
+    norm = scaled.CudaRmsNormQuantizePlan(name="p", columns=100)
+    for wrong in (weight.float(), weight[:99], torch.ones(200, dtype=torch.bfloat16, device=cuda_device)[::2], weight.cpu(), None):
+        with pytest.raises(ValueError, match="weight must"):
+            norm.invoke(executable, x, wrong, x)
+    with pytest.raises(ValueError, match="residual must"):
+        norm.invoke(executable, x, weight, x[:3])
+    with pytest.raises(ValueError, match="residual_out must"):
+        norm.invoke(executable, x, weight, x, residual_out=x.float())
+    matmul = scaled.CudaScaledMatmulPlan(name="p", n=32, k=256)
+    product = matmul.build(cuda_device)
+    lhs, lhs_scales = operand(1, 4, 256, cuda_device)
+    rhs, rhs_scales = operand(2, 32, 256, cuda_device)
+    for wrong in ((lhs[:, :255], lhs_scales, rhs, rhs_scales), (lhs, lhs_scales[:3], rhs, rhs_scales), (lhs, lhs_scales, rhs[:31], rhs_scales[:31]),
+                  (lhs, lhs_scales, rhs, rhs_scales[:, :1]), (lhs.view(torch.float8_e5m2), lhs_scales, rhs, rhs_scales),
+                  (lhs, lhs_scales.view(torch.uint8), rhs, rhs_scales), (lhs, lhs_scales.cpu(), rhs, rhs_scales)):
+        with pytest.raises(ValueError):
+            matmul.invoke(product, *wrong)
+    with pytest.raises(ValueError, match="out must"):
+        matmul.invoke(product, lhs, lhs_scales, rhs, rhs_scales, out=torch.zeros(4, 32, device=cuda_device))

@@ -72,66 +72,81 @@ def test_codes_get_the_pitch_the_matmul_wants(columns, pitch):
 
 
 class _Recorder:
-    """An executable that records what would be enqueued instead of calling the library."""
+    """An executable that records the binding calls instead of making them."""
 
-    device = torch.device("cpu")
+    index = 0
 
-    def __init__(self):
-        self.calls = []
+    def __init__(self, plan=None):
+        self.calls, self.plan, self.binding = [], plan, self
+        self.desc_address = self.status_address = 0
 
-    def quantize(self, *arguments):
+    def record(self, *arguments):
         self.calls.append(arguments)
+        return tuple(arguments[-2:])
 
-    rms_norm_quantize = enqueue = quantize
+    quantize_rows = rms_norm_quantize = scaled_matmul = record
 
 
-def test_invoke_refuses_wrong_operands():
+def test_invoke_refuses_what_a_plan_does_not_take():
     recorder = _Recorder()
-    plan = scaled.CudaQuantizeRowsPlan(name="p", columns=100)
-    x = torch.zeros(4, 100, dtype=torch.bfloat16)
-    for wrong in (x.float(), x[:, :99], x[0], x.t(), torch.zeros(4, 200, dtype=torch.bfloat16)[:, ::2], x[:1].expand(4, 100), None):
-        with pytest.raises(ValueError, match="x must"):
-            plan.invoke(recorder, wrong)
-    with pytest.raises(ValueError, match="codes must"):
-        plan.invoke(recorder, x, codes=torch.zeros(3, 100).to(torch.float8_e4m3fn))
-    with pytest.raises(ValueError, match="scales must"):
-        plan.invoke(recorder, x, scales=torch.zeros(4, 2).to(torch.float8_e8m0fnu))
-    gated = scaled.CudaQuantizeRowsPlan(name="p", columns=100, gate="silu")
-    with pytest.raises(ValueError, match="x must"):
-        gated.invoke(recorder, x)
-
+    x, weight = torch.zeros(4, 100, dtype=torch.bfloat16), torch.ones(100, dtype=torch.bfloat16)
     norm = scaled.CudaRmsNormQuantizePlan(name="p", columns=100)
-    weight = torch.ones(100, dtype=torch.bfloat16)
     with pytest.raises(ValueError, match="residual"):
         norm.invoke(recorder, x, weight)
-    with pytest.raises(ValueError, match="weight"):
-        norm.invoke(recorder, x, weight.float(), x)
-    with pytest.raises(ValueError, match="weight"):
-        norm.invoke(recorder, x, torch.ones(200, dtype=torch.bfloat16)[::2], x)
-    with pytest.raises(ValueError, match="residual must"):
-        norm.invoke(recorder, x, weight, x[:3])
     plain = scaled.CudaRmsNormQuantizePlan(name="p", columns=100, with_residual=False)
     with pytest.raises(ValueError, match="residual"):
         plain.invoke(recorder, x, weight, x)
     with pytest.raises(ValueError, match="residual_out"):
         plain.invoke(recorder, x, weight, residual_out=x)
-
     matmul = scaled.CudaScaledMatmulPlan(name="p", n=32, k=256)
-    recorder.plan = scaled.CudaScaledMatmulPlan(name="p", n=32, k=512)
     with pytest.raises(ValueError, match="another plan"):
-        matmul.invoke(recorder, None, None, None, None)
-    recorder.plan = scaled.CudaScaledMatmulPlan(name="p", n=32, k=256)
-    codes, scales = torch.zeros(4, 256).to(torch.float8_e4m3fn), torch.ones(4, 2).to(torch.float8_e8m0fnu)
-    rhs, rhs_scales = torch.zeros(32, 256).to(torch.float8_e4m3fn), torch.ones(32, 2).to(torch.float8_e8m0fnu)
-    for wrong in ((codes[:, :255], scales, rhs, rhs_scales), (codes, scales[:3], rhs, rhs_scales), (codes, scales, rhs[:31], rhs_scales[:31]),
-                  (codes, scales, rhs, rhs_scales[:, :1]), (codes.view(torch.float8_e5m2), scales, rhs, rhs_scales),
-                  (codes, scales.view(torch.uint8), rhs, rhs_scales)):
-        with pytest.raises(ValueError):
-            matmul.invoke(recorder, *wrong)
-    with pytest.raises(ValueError, match="out must"):
-        matmul.invoke(recorder, codes, scales, rhs, rhs_scales, out=torch.zeros(4, 32))
+        matmul.invoke(_Recorder(scaled.CudaScaledMatmulPlan(name="p", n=32, k=512)), None, None, None, None)
     assert not recorder.calls
-    assert tuple(matmul.invoke(recorder, codes, scales, rhs, rhs_scales).shape) == (4, 32) and len(recorder.calls) == 1
+    norm.invoke(recorder, x, weight, x)
+    same = _Recorder(scaled.CudaScaledMatmulPlan(name="p", n=32, k=256))
+    matmul.invoke(same, 1, 2, 3, 4)
+    assert len(recorder.calls) == 1 and same.calls == [(0, 0, 0, 1, 2, 3, 4, None)]
+
+
+F32, BF16, CODES, SCALES = 0, 1, 3, 4
+
+
+def test_row_operands_are_checked():
+    check = _native.load_torch_binding().check_rows
+    x = torch.zeros(4, 100, dtype=torch.bfloat16)
+    assert check(x, 100, BF16, "x", -1, -1) == (4, 100) and check(x[::2], 100, BF16, "x", -1, 2) == (2, 200)
+    assert check(x[:1].expand(1, 100), 100, BF16, "x", -1, 1)[0] == 1 and check(x[:0], 100, BF16, "x", -1, -1)[0] == 0
+    assert check(torch.zeros(3, 7).to(torch.float8_e4m3fn), 7, CODES, "codes", -1, 3) == (3, 7)
+    assert check(torch.ones(3, 2).to(torch.float8_e8m0fnu), 2, SCALES, "scales", -1, 3) == (3, 2)
+    for wrong in (x.float(), x[:, :99], x[0], x.t(), x[None], None, 7, x.to_sparse()):
+        with pytest.raises(ValueError, match="x must be a BFloat16 tensor of shape"):
+            check(wrong, 100, BF16, "x", -1, -1)
+    with pytest.raises(ValueError, match=r"out must be a Float tensor of shape \(5, 100\)"):
+        check(x.float(), 100, F32, "out", -1, 5)
+    for wrong in (torch.zeros(4, 200, dtype=torch.bfloat16)[:, ::2], x[:1].expand(4, 100), torch.zeros(400, dtype=torch.bfloat16).as_strided((4, 100), (99, 1))):
+        with pytest.raises(ValueError, match="contiguous rows that do not overlap"):
+            check(wrong, 100, BF16, "x", -1, -1)
+    with pytest.raises(ValueError, match="x must be on cuda:0"):
+        check(x, 100, BF16, "x", 0, -1)
+    with pytest.raises(TypeError, match="6 arguments"):
+        check(x)
+
+
+def test_binding_calls_refuse_tensors_that_are_not_on_the_device():
+    binding = _native.load_torch_binding()
+    x, weight = torch.zeros(4, 100, dtype=torch.bfloat16), torch.ones(100, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="x must be on cuda:0"):
+        binding.quantize_rows(0, x, 100, BF16, 0, None, None)
+    with pytest.raises(ValueError, match="x must be a BFloat16 tensor of shape .rows, 200."):
+        binding.quantize_rows(0, x, 100, BF16, 1, None, None)
+    with pytest.raises(ValueError, match="x must be on cuda:0"):
+        binding.rms_norm_quantize(0, x, 100, BF16, weight, BF16, 1e-5, x, None, None, None)
+    desc = _native.ScaledMatmulDesc(n=32, k=100, out_dtype=1, tile=0, k_split=0)
+    with pytest.raises(ValueError, match="lhs must be a Float8_e4m3fn tensor"):
+        binding.scaled_matmul(0, ctypes.addressof(desc), 0, x, None, None, None, None)
+    for call in (binding.quantize_rows, binding.rms_norm_quantize, binding.scaled_matmul, binding.init):
+        with pytest.raises(TypeError, match="arguments"):
+            call()
 
 
 def _quantize(**overrides):

@@ -228,6 +228,32 @@ def load() -> ctypes.CDLL:
     return lib
 
 
+_torch_binding = None
+
+
+def load_torch_binding():
+    """The compiled module that calls the 8-bit layer's entry points on torch tensors (csrc/torch_binding.cpp),
+    bound to the loaded library. As the library, it is built by ``__graft_entry__.build()`` and has no fallback."""
+    global _torch_binding
+    if _torch_binding is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  its libraries have to be loaded first
+
+        path = PACKAGE_DIR / "lib" / "cake_torch_binding.so"
+        if not path.exists():
+            raise ImportError(f"{path} is missing: build it first (python -c 'import __graft_entry__ as g; g.build()')")
+        loader = importlib.machinery.ExtensionFileLoader("cake_torch_binding", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("cake_torch_binding", loader))
+        loader.exec_module(module)
+        lib = load()
+        module.init(*(ctypes.cast(entry, ctypes.c_void_p).value
+                      for entry in (lib.cake_quantize_rows_enqueue, lib.cake_rms_norm_quantize_enqueue, lib.cake_scaled_matmul_enqueue)))
+        _torch_binding = module
+    return _torch_binding
+
+
 def check(code: int) -> None:
     """Raises CakeError with the library's message for a non-zero status."""
     if code != CAKE_OK:

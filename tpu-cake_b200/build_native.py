@@ -69,6 +69,30 @@ def build(*, force: bool = False, verbose: bool = False) -> Path:
     return LIBRARY
 
 
+TORCH_BINDING = LIB_DIR / "cake_torch_binding.so"
+
+
+def build_torch_binding(*, force: bool = False) -> Path:
+    """Compiles ``csrc/torch_binding.cpp``, the Python module that checks torch tensors and calls the 8-bit
+    layer's entry points, against the headers of the torch that runs this."""
+    import sysconfig
+
+    import torch
+
+    LIB_DIR.mkdir(exist_ok=True)
+    source = CSRC / "torch_binding.cpp"
+    if force or _stale(TORCH_BINDING, [source, PACKAGE_DIR.parent / "include" / "cake_abi.h"]):
+        root = Path(torch.__file__).resolve().parent
+        cuda = Path(_nvcc()).resolve().parent.parent
+        includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include", Path(sysconfig.get_paths()["include"])]
+        cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+               *(f"-I{path}" for path in includes), str(source), "-o", str(TORCH_BINDING), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+        result = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+        if result.returncode != 0:
+            raise RuntimeError(f"g++ failed for {source.name}:\n{result.stdout}")
+    return TORCH_BINDING
+
+
 PUSH_RATE_PROGRAM = LIB_DIR / "peer_push_rate"
 
 
@@ -88,4 +112,5 @@ def build_push_rate_program(*, force: bool = False) -> Path:
 if __name__ == "__main__":
     path = build(force="--force" in sys.argv, verbose="--verbose" in sys.argv or bool(os.environ.get("CAKE_VERBOSE")))
     print(path)
+    print(build_torch_binding(force="--force" in sys.argv))
     print(build_push_rate_program(force="--force" in sys.argv))

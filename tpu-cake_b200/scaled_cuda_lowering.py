@@ -31,7 +31,6 @@ GROUP_COLUMNS = 128
 CODE_DTYPE = torch.float8_e4m3fn
 SCALE_DTYPE = torch.float8_e8m0fnu
 MAX_NORM_COLUMNS = 32768
-_DTYPES = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
 _CAKE_DTYPES = {"bf16": _native.CAKE_DTYPE_BF16, "f16": _native.CAKE_DTYPE_F16, "f32": _native.CAKE_DTYPE_F32}
 _GATES = {"none": _native.CAKE_GATE_NONE, "silu": _native.CAKE_GATE_SILU}
 
@@ -53,68 +52,28 @@ def empty_scales(rows: int, columns: int, device: torch.device) -> torch.Tensor:
     return torch.empty(rows, -(-columns // GROUP_COLUMNS), dtype=SCALE_DTYPE, device=device)
 
 
-def _rows(tensor, columns: int, dtype: torch.dtype, name: str, device: torch.device, rows: int | None = None) -> tuple[int, int]:
-    """Checks a row operand (contiguous rows, any row stride that does not overlap); returns its rows and
-    row stride. A call's time on the host is its time, for few rows: the good case is one expression."""
-    if isinstance(tensor, torch.Tensor) and tensor.dtype is dtype:
-        shape, strides = tensor.shape, tensor.stride()
-        if len(shape) == 2 and shape[1] == columns and (rows is None or shape[0] == rows):
-            if tensor.device != device:
-                raise ValueError(f"{name} must be on {device}, is on {tensor.device}")
-            if (columns > 1 and strides[1] != 1) or (shape[0] > 1 and strides[0] < columns):
-                raise ValueError(f"{name} must have contiguous rows that do not overlap, got strides {strides}")
-            return shape[0], strides[0]
-    got = (tuple(tensor.shape), tensor.dtype) if isinstance(tensor, torch.Tensor) else type(tensor)
-    raise ValueError(f"{name} must be a {dtype} tensor of shape {('rows' if rows is None else rows, columns)}, got {got}")
-
-
-class _Executable:
-    """The library and the device a plan was built on."""
+class RowQuantizeExecutable:
+    """What a plan runs on: a device and the compiled binding. The row kernels keep nothing else."""
 
     def __init__(self, device: torch.device):
-        self._lib = _native.load()
-        self.device = torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)
-        self._index = self.device.index
-
-    def _call(self, entry, *arguments) -> None:
-        """Enqueues on the device's current stream. The library launches on the current device."""
-        # The raw handle: torch.cuda.current_stream builds a Stream object, 3 us of a 15 us call.
-        stream = torch._C._cuda_getCurrentRawStream(self._index)
-        if torch._C._cuda_getDevice() == self._index:
-            code = entry(*arguments, stream)
-        else:
-            with torch.cuda.device(self.device):
-                code = entry(*arguments, stream)
-        if code != _native.CAKE_OK:
-            _native.check(code)
+        self.binding = _native.load_torch_binding()
+        self.index = torch.cuda.current_device() if device.index is None else device.index
+        self.device = torch.device("cuda", self.index)
 
     def close(self) -> None:
         """Nothing to release: here for the executables' common surface."""
 
 
-class RowQuantizeExecutable(_Executable):
-    """The row kernels keep nothing: a device and the library."""
-
-    def quantize(self, *arguments) -> None:
-        self._call(self._lib.cake_quantize_rows_enqueue, *arguments)
-
-    def rms_norm_quantize(self, *arguments) -> None:
-        self._call(self._lib.cake_rms_norm_quantize_enqueue, *arguments)
-
-
-class ScaledMatmulExecutable(_Executable):
+class ScaledMatmulExecutable(RowQuantizeExecutable):
     """A matmul plan's descriptor and its status word on a GPU."""
 
     def __init__(self, plan: "CudaScaledMatmulPlan", desc: _native.ScaledMatmulDesc, device: torch.device):
         super().__init__(device)
         self.plan = plan
         self._desc = desc
-        self._desc_address = ctypes.addressof(desc)
+        self.desc_address = ctypes.addressof(desc)
         self._status = torch.zeros(4, dtype=torch.int32).to(self.device)  # there when the copy returns, for any stream
-        self._status_address = self._status.data_ptr()
-
-    def enqueue(self, *arguments) -> None:
-        self._call(self._lib.cake_scaled_matmul_enqueue, self._desc_address, *arguments, self._status_address)
+        self.status_address = self._status.data_ptr()
 
     def status(self) -> tuple[int, int, int, int]:
         """Waits for the current stream's work and reads the status word; raises if a bounded wait ran out."""
@@ -125,19 +84,11 @@ class ScaledMatmulExecutable(_Executable):
         return (code, *details)
 
 
-def _outputs(codes, scales, rows: int, columns: int, device: torch.device):
-    """Codes and scales of a row operator with their row strides: the caller's, checked, or new ones."""
-    if codes is None:
-        codes = empty_codes(rows, columns, device)
-        codes_stride = -(-columns // 128) * 128
-    else:
-        _, codes_stride = _rows(codes, columns, CODE_DTYPE, "codes", device, rows)
-    groups = -(-columns // GROUP_COLUMNS)
-    if scales is None:
-        scales, scales_stride = torch.empty(rows, groups, dtype=SCALE_DTYPE, device=device), groups
-    else:
-        _, scales_stride = _rows(scales, groups, SCALE_DTYPE, "scales", device, rows)
-    return codes, scales, codes_stride, scales_stride
+def _outputs(result):
+    """A binding call's outputs; its error code raises."""
+    if type(result) is int:
+        _native.check(result)
+    return result
 
 
 def _source(kind: str, kernel: str, plan, fields: tuple[str, ...]) -> str:
@@ -163,8 +114,8 @@ class CudaQuantizeRowsPlan:
     def __post_init__(self) -> None:
         if self.columns < 1:
             raise ValueError(f"columns must be positive, got {self.columns}")
-        if self.input_dtype not in _DTYPES:
-            raise ValueError(f"input dtype must be one of {tuple(_DTYPES)}, got {self.input_dtype}")
+        if self.input_dtype not in _CAKE_DTYPES:
+            raise ValueError(f"input dtype must be one of {tuple(_CAKE_DTYPES)}, got {self.input_dtype}")
         if self.gate not in _GATES:
             raise ValueError(f"gate must be one of {tuple(_GATES)}, got {self.gate}")
 
@@ -178,12 +129,7 @@ class CudaQuantizeRowsPlan:
         return RowQuantizeExecutable(_device(device))
 
     def invoke(self, executable: RowQuantizeExecutable, x, *, codes=None, scales=None) -> tuple[torch.Tensor, torch.Tensor]:
-        device, columns = executable.device, self.columns
-        rows, stride = _rows(x, columns if self.gate == "none" else 2 * columns, _DTYPES[self.input_dtype], "x", device)
-        codes, scales, codes_stride, scales_stride = _outputs(codes, scales, rows, columns, device)
-        executable.quantize(x.data_ptr(), _CAKE_DTYPES[self.input_dtype], stride, _GATES[self.gate], rows, columns,
-                            codes.data_ptr(), codes_stride, scales.data_ptr(), scales_stride)
-        return codes, scales
+        return _outputs(executable.binding.quantize_rows(executable.index, x, self.columns, _CAKE_DTYPES[self.input_dtype], _GATES[self.gate], codes, scales))
 
 
 @dataclass(frozen=True)
@@ -201,8 +147,8 @@ class CudaRmsNormQuantizePlan:
     def __post_init__(self) -> None:
         if not 1 <= self.columns <= MAX_NORM_COLUMNS:
             raise ValueError(f"a norm's row is held on chip: columns must be 1 to {MAX_NORM_COLUMNS}, got {self.columns}")
-        if self.input_dtype not in _DTYPES:
-            raise ValueError(f"input dtype must be one of {tuple(_DTYPES)}, got {self.input_dtype}")
+        if self.input_dtype not in _CAKE_DTYPES:
+            raise ValueError(f"input dtype must be one of {tuple(_CAKE_DTYPES)}, got {self.input_dtype}")
         if self.weight_dtype not in (self.input_dtype, "f32"):
             raise ValueError(f"weight dtype must be the input's or f32, got {self.weight_dtype}")
         if not self.epsilon >= 0:
@@ -220,28 +166,12 @@ class CudaRmsNormQuantizePlan:
 
     def invoke(self, executable: RowQuantizeExecutable, x, weight, residual=None, *, codes=None, scales=None, residual_out=None):
         """Returns (codes, scales, new residual or None). ``residual_out`` may be ``residual`` or ``x``."""
-        device, columns, dtype = executable.device, self.columns, _DTYPES[self.input_dtype]
-        rows, stride = _rows(x, columns, dtype, "x", device)
-        if not isinstance(weight, torch.Tensor) or weight.dtype != _DTYPES[self.weight_dtype] or weight.shape != (columns,) \
-                or weight.device != device or (columns > 1 and weight.stride(0) != 1):
-            raise ValueError(f"weight must be a contiguous {self.weight_dtype} vector of {columns} on {device}")
         if (residual is not None) != self.with_residual:
             raise ValueError("residual must be given to a plan with residual, and to no other")
-        residual_ptr, residual_stride, out_ptr, out_stride = None, 0, None, 0
-        if residual is not None:
-            _, residual_stride = _rows(residual, columns, dtype, "residual", device, rows)
-            if residual_out is None:
-                residual_out, out_stride = torch.empty(rows, columns, dtype=dtype, device=device), columns
-            else:
-                _, out_stride = _rows(residual_out, columns, dtype, "residual_out", device, rows)
-            residual_ptr, out_ptr = residual.data_ptr(), residual_out.data_ptr()
-        elif residual_out is not None:
+        if residual is None and residual_out is not None:
             raise ValueError("residual_out needs a plan with residual")
-        codes, scales, codes_stride, scales_stride = _outputs(codes, scales, rows, columns, device)
-        executable.rms_norm_quantize(x.data_ptr(), _CAKE_DTYPES[self.input_dtype], stride, residual_ptr, residual_stride, out_ptr, out_stride,
-                                     weight.data_ptr(), _CAKE_DTYPES[self.weight_dtype], self.epsilon, rows, columns,
-                                     codes.data_ptr(), codes_stride, scales.data_ptr(), scales_stride)
-        return codes, scales, residual_out
+        return _outputs(executable.binding.rms_norm_quantize(executable.index, x, self.columns, _CAKE_DTYPES[self.input_dtype], weight,
+                                                             _CAKE_DTYPES[self.weight_dtype], self.epsilon, residual, codes, scales, residual_out))
 
 
 @dataclass(frozen=True)
@@ -281,18 +211,8 @@ class CudaScaledMatmulPlan:
     def invoke(self, executable: ScaledMatmulExecutable, lhs, lhs_scales, rhs, rhs_scales, *, out=None) -> torch.Tensor:
         if executable.plan is not self and executable.plan != self:
             raise ValueError(f"the executable was built from another plan: {executable.plan}")
-        device, groups, dtype = executable.device, scale_columns(self.k), _DTYPES[self.output_dtype]
-        m, lhs_stride = _rows(lhs, self.k, CODE_DTYPE, "lhs", device)
-        _, lhs_scales_stride = _rows(lhs_scales, groups, SCALE_DTYPE, "lhs_scales", device, m)
-        _, rhs_stride = _rows(rhs, self.k, CODE_DTYPE, "rhs", device, self.n)
-        _, rhs_scales_stride = _rows(rhs_scales, groups, SCALE_DTYPE, "rhs_scales", device, self.n)
-        if out is None:
-            out, out_stride = torch.empty(m, self.n, dtype=dtype, device=device), self.n
-        else:
-            _, out_stride = _rows(out, self.n, dtype, "out", device, m)
-        executable.enqueue(m, lhs.data_ptr(), lhs_stride, lhs_scales.data_ptr(), lhs_scales_stride, rhs.data_ptr(), rhs_stride,
-                           rhs_scales.data_ptr(), rhs_scales_stride, out.data_ptr(), out_stride)
-        return out
+        return _outputs(executable.binding.scaled_matmul(executable.index, executable.desc_address, executable.status_address,
+                                                         lhs, lhs_scales, rhs, rhs_scales, out))
 
 
 @dataclass(frozen=True)
