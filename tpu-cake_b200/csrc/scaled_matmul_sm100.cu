@@ -776,15 +776,16 @@ bool is_narrow(int tile) { return tile <= 128; }
 // Nanoseconds that a call of this shape is expected to take, from times measured at 1 to 1024 rows and
 // extents of 1024 to 8192 (graph replays, one after the other): good to about a fifth, and the neighbours of the
 // least are within that of each other. Some 4000 pass before the first and after the last k block.
-double narrow_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int split, int sm_count) {
+// `lines`: operand rows start on 128-byte lines; otherwise each of a block's 128-byte rows is two requests to L2.
+double narrow_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int split, int sm_count, bool lines) {
   const double blocks = static_cast<double>((n + 127) / 128) * ((m + tile - 1) / tile) * split;
   const double kb = static_cast<double>((k_blocks + split - 1) / split);
   // One k block of one block's: what the tensor core takes for 128 x 64 or less, more with the bytes that the
   // SM has to fetch for it (and for the block it shares the SM with).
   const bool alone = blocks <= sm_count;
-  const double k_block = tile <= 32 ? (alone ? 210 : 235) : tile == 64 ? (alone ? 245 : 330) : (alone ? 345 : 430);
+  const double k_block = (tile <= 32 ? (alone ? 210 : 235) : tile == 64 ? (alone ? 245 : 330) : (alone ? 345 : 430)) * (lines ? 1 : 1.5);
   const double waves = std::ceil(blocks / (2.0 * sm_count));
-  const double fetch = blocks * kb * (16384 + 128.0 * tile) / 17000;
+  const double fetch = blocks * kb * (16384 + 128.0 * tile) / (lines ? 17000 : 11300);
   // HBM at 5.0 TB/s with one block's ring in flight per SM, 6.2 with two; less if several blocks want the same rows.
   const double hbm = static_cast<double>(n) * k_blocks * 128 / (alone ? 5000 : 6200) * (m > tile ? 1.25 : 1);
   const double sharing = split > 1 ? waves * split * (200 + 6.0 * tile) : 0;
@@ -793,16 +794,16 @@ double narrow_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int split, in
 
 // tensor_store: the output's rows are whole 16-byte pieces. Other rows leave 64 bytes at a time, most of them
 // parts of 32-byte sectors: four times as slow (1001 x 5120 x 4096: 21 us, x 4099: 29 us).
-double wide_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int sm_count, bool tensor_store) {
+double wide_ns(int64_t m, int64_t n, int64_t k_blocks, int tile, int sm_count, bool lines, bool tensor_store) {
   const double tiles = static_cast<double>((m + 255) / 256) * ((n + tile - 1) / tile), pairs = sm_count / 2;
   const double waves = std::ceil(tiles / pairs);
-  const double main_loop = k_blocks * (60 + 1.07 * tile) * (tiles > 0.6 * pairs ? 1.18 : 1);  // L2 is shared by as many
+  const double main_loop = k_blocks * (60 + 1.07 * tile) * (tiles > 0.6 * pairs ? 1.18 : 1) * (lines ? 1 : 1.25);  // L2 is shared by as many
   const double epilogue = tile * (tensor_store ? 10 : 38);
   // 256 columns leave no second accumulator, so nothing hides a tile's epilogue.
   return 4500 + (tile == 256 ? waves * (main_loop + epilogue) : waves * std::max(main_loop, epilogue) + epilogue);
 }
 
-Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count, bool tensor_store) {
+Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count, bool lines, bool tensor_store) {
   Choice best = {d.tile, d.k_split};
   const int64_t k_blocks = (d.k + cake::kBlockK - 1) / cake::kBlockK;
   double least = 0;
@@ -810,7 +811,8 @@ Choice choose(const cake_scaled_matmul_desc& d, int64_t m, int sm_count, bool te
     if (d.tile != 0 && tile != d.tile) continue;
     for (int split : {1, 2, 4, 8}) {
       if (split > 1 && (!is_narrow(tile) || split > k_blocks || (d.k_split != 0 && d.tile != 0))) break;
-      const double ns = is_narrow(tile) ? narrow_ns(m, d.n, k_blocks, tile, split, sm_count) : wide_ns(m, d.n, k_blocks, tile, sm_count, tensor_store);
+      const double ns = is_narrow(tile) ? narrow_ns(m, d.n, k_blocks, tile, split, sm_count, lines)
+                                     : wide_ns(m, d.n, k_blocks, tile, sm_count, lines, tensor_store);
       if (least == 0 || ns < least) {
         least = ns;
         best = {tile, split};
@@ -846,7 +848,7 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
   const int osize = d.out_dtype == CAKE_DTYPE_F32 ? 4 : 2;
   const int64_t k_blocks = (d.k + cake::kBlockK - 1) / cake::kBlockK;
   // With a single row its stride says nothing; tensor maps still want a valid one.
-  const int64_t pitch = (d.k + 15) / 16 * 16;
+  const int64_t pitch = (d.k + 127) / 128 * 128;
   if (m == 1) {
     lhs_row_stride = pitch;
     out_row_stride = d.n;
@@ -870,7 +872,8 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
   // Tensor stores write whole 16-byte pieces, also where the row ends inside one: only rows of whole pieces
   // leave what lies behind them alone.
   const bool tensor_store = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && out_row_stride * osize % 16 == 0 && d.n * osize % 16 == 0;
-  const Choice c = choose(d, m, device.sm_count, tensor_store);
+  const bool lines = ((reinterpret_cast<uintptr_t>(lhs) | reinterpret_cast<uintptr_t>(rhs) | static_cast<uintptr_t>(lhs_row_stride) | static_cast<uintptr_t>(rhs_row_stride)) & 127) == 0;
+  const Choice c = choose(d, m, device.sm_count, lines, tensor_store);
   const bool narrow = is_narrow(c.tile);
   cake::Params p;
   memset(&p, 0, sizeof(p));
