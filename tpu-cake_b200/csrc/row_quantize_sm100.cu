@@ -380,7 +380,30 @@ struct NormParams {
   uint32_t rows;
   int32_t cols;
   float epsilon;
+  double inverse_cols;
 };
+
+// 1 / sqrt(a) as the sum of two f32: the f32 value by one Newton-Raphson step in double. A value next to the border
+// of two codes goes to the wrong one by any error of the scale, and the whole row has the scale's; one step
+// in double costs six operations a thread. Zero and infinity pass through (their step is not a number).
+__device__ __forceinline__ void inverse_root(double a, float& hi, float& lo) {
+  const float y = 1.f / sqrtf(static_cast<float>(a));
+  hi = y;
+  lo = 0.f;
+  if (y > 0.f && y < __int_as_float(0x7F800000)) {
+    const double z = y, root = z + 0.5 * z * fma(-a * z, z, 1.0);
+    hi = static_cast<float>(root);
+    lo = static_cast<float>(root - hi);
+  }
+}
+
+// h (hi + lo) w with one rounding: the first product's own error, from a fused multiply-add, and what lo adds
+// go into the second.
+__device__ __forceinline__ F2 scaled(F2 h, F2 hi, F2 minus_hi, F2 lo, F2 w) {
+  const F2 product = mul2(h, hi);
+  const F2 rest = fma2(h, lo, fma2(h, hi, mul2(h, minus_hi)));
+  return fma2(product, w, mul2(rest, w));
+}
 
 // THREADS threads hold one row in registers, UNITS units of 16 elements each (unit i * THREADS + t of the row:
 // eight units are a group), so the sum x + residual is normalised as it is in 32 bits while its rounding is
@@ -390,7 +413,7 @@ template <typename T, typename W, int THREADS, int UNITS, bool VEC>
 __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_quantize_sm100(const __grid_constant__ NormParams p) {
   constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;  // rows of a block
   constexpr int kWarps = THREADS / 32;                      // warps of a row
-  __shared__ float partial[kRows][kWarps];
+  __shared__ double partial[kRows][kWarps];
   grid_dependency_wait();
   grid_dependency_trigger();
   const int t = threadIdx.x % THREADS;
@@ -436,17 +459,20 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
       for (int e = 0; e < kVec / 2; ++e) squares = fma2(h[i][k][e], h[i][k][e], squares);
   float even, odd;
   unpack2(squares, even, odd);
-  float sum = even + odd;
+  // 16 UNITS squares a thread in f32; between threads in double, where a rounding would be the whole row's.
+  double sum = static_cast<double>(even) + odd;
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   if (kWarps > 1) {
     if ((t & 31) == 0) partial[r][t / 32] = sum;
     __syncthreads();
-    sum = (t & 31) < kWarps ? partial[r][t & 31] : 0.f;
+    sum = (t & 31) < kWarps ? partial[r][t & 31] : 0.0;
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
   }
-  const float scale = 1.f / sqrtf(sum / static_cast<float>(p.cols) + p.epsilon);
+  float hi, lo;
+  inverse_root(sum * p.inverse_cols + static_cast<double>(p.epsilon), hi, lo);
+  const F2 hi2 = pack2(hi, hi), minus_hi2 = pack2(-hi, -hi), lo2 = pack2(lo, lo);
 #pragma unroll
   for (int i = 0; i < UNITS; ++i) {
     float magnitude = 0.f;
@@ -457,7 +483,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
       load_raw<W, VEC>(weight, static_cast<const W*>(p.weight) + col, valid_at<VEC>(col, p.cols));
 #pragma unroll
       for (int e = 0; e < kVec / 2; ++e) {
-        h[i][k][e] = mul2(mul2(h[i][k][e], pack2(scale, scale)), widen<W>(weight, e));
+        h[i][k][e] = scaled(h[i][k][e], hi2, minus_hi2, lo2, widen<W>(weight, e));
         magnitude = largest_abs(magnitude, h[i][k][e]);
       }
     }
@@ -610,6 +636,7 @@ int32_t cake_rms_norm_quantize_enqueue(const void* x, int32_t dtype, int64_t x_r
   p.rows = static_cast<uint32_t>(rows);
   p.cols = static_cast<int32_t>(cols);
   p.epsilon = epsilon;
+  p.inverse_cols = 1.0 / static_cast<double>(cols);
   const bool strides = rows == 1 || (x_row_stride * size % 16 == 0 && q_row_stride % 8 == 0 &&
                                      (!residual || (residual_row_stride * size % 16 == 0 && residual_out_row_stride * size % 16 == 0)));
   const bool vec = cols % kVec == 0 && strides && aligned(x, 16) && aligned(residual, 16) && aligned(residual_out, 16) && aligned(weight, 16) && aligned(q, 8);
