@@ -120,7 +120,7 @@ __device__ __forceinline__ bool wait_or_abort(uint32_t bar, uint32_t parity, vol
 }
 
 // The scale bytes of COUNT operand rows for 16 k blocks, from k block kb on, as four words each; anything past
-// the last k block. `align`: the rows' addresses and kb are multiples of it (16, 4 or 1). Every branch is the
+// the last k block. `align`: the rows' addresses and kb are multiples of it (16, 8, 4 or 1). Every branch is the
 // whole warp's and has all rows' loads inside, so that they are under way together. Ordinary loads: this kernel
 // may have started before the one that writes the scales ended, so they are not read-only for its lifetime.
 template <int COUNT>
@@ -133,6 +133,17 @@ __device__ __forceinline__ void load_scales(uint32_t (&w)[COUNT][4], const uint8
       w[r][1] = v.y;
       w[r][2] = v.z;
       w[r][3] = v.w;
+    }
+    return;
+  }
+  if (align >= 8 && kb + 16 <= k_blocks) {
+#pragma unroll
+    for (int r = 0; r < COUNT; ++r) {
+      const uint2 lo = *reinterpret_cast<const uint2*>(row[r] + kb), hi = *reinterpret_cast<const uint2*>(row[r] + kb + 8);
+      w[r][0] = lo.x;
+      w[r][1] = lo.y;
+      w[r][2] = hi.x;
+      w[r][3] = hi.y;
     }
     return;
   }
@@ -159,7 +170,7 @@ __device__ __forceinline__ void load_scales(uint32_t (&w)[COUNT][4], const uint8
 
 __device__ __forceinline__ int scale_alignment(const uint8_t* scales, int64_t stride, int kb_begin) {
   const uintptr_t bits = reinterpret_cast<uintptr_t>(scales) | static_cast<uintptr_t>(stride) | static_cast<uintptr_t>(kb_begin);
-  return (bits & 15) == 0 ? 16 : (bits & 3) == 0 ? 4 : 1;
+  return (bits & 15) == 0 ? 16 : (bits & 7) == 0 ? 8 : (bits & 3) == 0 ? 4 : 1;
 }
 
 // Consecutive tiles walk 8 row tiles down before moving one column tile right, so that the blocks of a
@@ -205,6 +216,58 @@ __device__ __forceinline__ void store_tokens(char* at, int64_t stride, const uin
     for (int j = 0; j < 16; ++j, at += stride)
       if (j < tokens) store_as(at, v[j], T());
   }
+}
+
+// The accumulator has been read: one arrival of four (eight in a pair) on the issuing block's barrier.
+__device__ __forceinline__ void release_accumulator(uint64_t* bar, int lane) {
+  tcgen05_fence_before();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_remote(cluster_addr(smem_u32(bar), 0));
+}
+
+// The warp's staging slot that comes next, once the store that had it has read it.
+__device__ __forceinline__ uint8_t* next_slot(const Params& p, uint8_t* staging, int& staged, int lane) {
+  uint8_t* slot = staging + (staged % kStagingSlots) * kStagingBytes;
+  if (p.tma_store && staged >= kStagingSlots) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStagingSlots - 1) : "memory");
+    __syncwarp();
+  }
+  ++staged;
+  return slot;
+}
+
+// Staged boxes of 32 rows x 32 columns of T to the output.
+template <typename T>
+__device__ __forceinline__ void leave(const Params& p, const CUtensorMap& map, const uint8_t* slot, int row0, int col, int boxes, int lane) {
+  if (p.tma_store) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      for (int b = 0; b < boxes; ++b) {
+        if (col + 32 * b < p.rows_b)
+          asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
+                       ::"l"(reinterpret_cast<uint64_t>(&map)), "r"(smem_u32(slot + b * 32 * 32 * sizeof(T))), "r"(col + 32 * b), "r"(row0)
+                       : "memory");
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    return;
+  }
+  // Rows whose pitch, base or length is not a multiple of 16 bytes: one row of 32 columns per store.
+  __syncwarp();
+  const int rows = min(32, p.rows_a - row0);
+  for (int b = 0; b < boxes; ++b) {
+    const int c = col + 32 * b + lane;
+    if (c < p.rows_b) {
+      T* dst = static_cast<T*>(p.out) + static_cast<int64_t>(row0) * p.out_stride + c;
+      const uint8_t* box = slot + b * 32 * 32 * sizeof(T);
+      for (int r = 0; r < rows; ++r, dst += p.out_stride) {
+        const int piece = sizeof(T) == 4 ? (lane >> 2) ^ (r & 7) : (lane >> 3) ^ ((r >> 1) & 3);
+        *dst = reinterpret_cast<const T*>(box + r * 32 * sizeof(T) + piece * 16)[lane % (16 / sizeof(T))];
+      }
+    }
+  }
+  __syncwarp();
 }
 
 // This block's share of a tile's pieces (one token, four columns): the sums over the cluster's blocks in rank
@@ -511,8 +574,8 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------------ scales
-    // 16 k blocks at a time: the fence and the arrival at cluster scope take some 1500 cycles, which a word
-    // at a time was more than its four k blocks' MMAs. Rows past an operand's end (and past the tile's)
+    // 16 k blocks at a time: one fence and one arrival for four words, and few loads, each of which touches a
+    // line per operand row. A word at a time, all of it took longer than the word's MMAs. Rows past an operand's end (and past the tile's)
     // get the last row's scales: their codes are zeros, or not there, and what comes of them is not stored.
     const int align = min(scale_alignment(p.scales_a, p.scales_a_stride, kb_begin), scale_alignment(p.scales_b, p.scales_b_stride, kb_begin));
     constexpr int kRowsOfB = (BN + 31) / 32;
@@ -549,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
         fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) {
-          if (PAIR) mbar_arrive_cluster(cluster_addr(smem_u32(&scale_full[slot]), 0));
+          if (PAIR) mbar_arrive_remote(cluster_addr(smem_u32(&scale_full[slot]), 0));
           else mbar_arrive(smem_u32(&scale_full[slot]));
         }
         if (++slot == kScaleSlots) {
@@ -603,66 +666,48 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
         tcgen05_fence_before();
         continue;
       }
-      // Wide: lane = output row, register = column. Chunks of 32 x 32 leave through shared memory, in the
-      // layout of a swizzled tensor store's box (64-byte rows of bf16, 128-byte rows of f32).
-      const int row_bytes = p.out_f32 ? 128 : 64;
+      // Wide: lane = output row, register = column. 32 rows x 128 bytes at a time (64 columns of bf16, as two
+      // boxes of 32, or 32 of f32) leave through shared memory, in the layout of a swizzled tensor store's box.
+      if (p.out_f32) {
 #pragma unroll 1
-      for (int c = 0; c < BN; c += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32b_x32(t_row + c, v);
-        tmem_ld_wait();
-        if (c == BN - 32) {
-          tcgen05_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(cluster_addr(smem_u32(&tmem_empty[buf]), 0));
-        }
-        const int col = tb * BN + c;
-        if (row0 >= p.rows_a || col >= p.rows_b) continue;  // warp-uniform
-        uint8_t* slot = my_staging + (staged % kStagingSlots) * kStagingBytes;
-        if (p.tma_store && staged >= kStagingSlots) {
-          if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kStagingSlots - 1) : "memory");
-          __syncwarp();
-        }
-        ++staged;
-        if (p.out_f32) {
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t_row + c, v);
+          tmem_ld_wait();
+          if (c == BN - 32) release_accumulator(&tmem_empty[buf], lane);
+          const int col = tb * BN + c;
+          if (row0 >= p.rows_a || col >= p.rows_b) continue;  // warp-uniform
+          uint8_t* slot = next_slot(p, my_staging, staged, lane);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             *reinterpret_cast<uint4*>(slot + lane * 128 + ((j ^ (lane & 7)) << 4)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(v[8 * j + 2 * e]), __uint_as_float(v[8 * j + 2 * e + 1]));
-            *reinterpret_cast<uint4*>(slot + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
-          }
+          leave<float>(p, map_out, slot, row0, col, 1, lane);
         }
-        if (p.tma_store) {
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];"
-                         ::"l"(reinterpret_cast<uint64_t>(&map_out)), "r"(smem_u32(slot)), "r"(col), "r"(row0)
-                         : "memory");
-            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-          }
-          continue;
-        }
-        // Rows whose pitch or base is not a multiple of 16 bytes: one row of 32 columns per store.
-        __syncwarp();
-        if (col + lane < p.rows_b) {
-          const int rows = min(32, p.rows_a - row0);
-          for (int r = 0; r < rows; ++r) {
-            const int64_t at = static_cast<int64_t>(row0 + r) * p.out_stride + col + lane;
-            if (p.out_f32) {
-              static_cast<float*>(p.out)[at] = *reinterpret_cast<const float*>(slot + r * row_bytes + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-            } else {
-              static_cast<__nv_bfloat16*>(p.out)[at] =
-                  *reinterpret_cast<const __nv_bfloat16*>(slot + r * row_bytes + (((lane >> 3) ^ ((r >> 1) & 3)) << 4) + (lane & 7) * 2);
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < BN; c += 64) {
+          const int boxes = c + 32 < BN ? 2 : 1;
+          uint32_t v[2][32];
+          tmem_ld_32x32b_x32(t_row + c, v[0]);
+          if (boxes == 2) tmem_ld_32x32b_x32(t_row + c + 32, v[1]);
+          tmem_ld_wait();
+          if (c + 64 >= BN) release_accumulator(&tmem_empty[buf], lane);
+          const int col = tb * BN + c;
+          if (row0 >= p.rows_a || col >= p.rows_b) continue;  // warp-uniform
+          uint8_t* slot = next_slot(p, my_staging, staged, lane);
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            if (b >= boxes) break;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              uint32_t w[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) w[e] = pack_bf16(__uint_as_float(v[b][8 * j + 2 * e]), __uint_as_float(v[b][8 * j + 2 * e + 1]));
+              *reinterpret_cast<uint4*>(slot + b * 2048 + lane * 64 + ((j ^ ((lane >> 1) & 3)) << 4)) = make_uint4(w[0], w[1], w[2], w[3]);
             }
           }
+          leave<__nv_bfloat16>(p, map_out, slot, row0, col, boxes, lane);
         }
-        __syncwarp();
       }
     }
     // Shared memory outlives every tensor store that still reads it.
