@@ -86,7 +86,7 @@ def build_torch_binding(*, force: bool = False) -> Path:
         cuda = Path(_nvcc()).resolve().parent.parent
         includes = [root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include", Path(sysconfig.get_paths()["include"])]
         cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-               *(f"-I{path}" for path in includes), str(source), "-o", str(TORCH_BINDING), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+               *(f"-I{path}" for path in includes), str(source), "-o", str(TORCH_BINDING), f"-L{root / 'lib'}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python"]
         result = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
         if result.returncode != 0:
             raise RuntimeError(f"g++ failed for {source.name}:\n{result.stdout}")

@@ -7,7 +7,7 @@
 // libcake_b200.so (init), so this module links against no kernel.
 #include <Python.h>
 
-#include <ATen/Functions.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -81,7 +81,7 @@ PyObject* output(PyObject* given, int64_t rows, int64_t cols, int64_t pitch, at:
     Py_INCREF(given);
     return given;
   }
-  at::Tensor t = at::empty_strided({rows, cols}, {pitch, 1}, at::TensorOptions().dtype(dtype).device(device));
+  at::Tensor t = at::detail::empty_strided_cuda({rows, cols}, {pitch, 1}, dtype, device);  // what torch.empty_strided comes to, without its dispatch
   out->data = t.data_ptr();
   out->count = rows;
   out->stride = pitch;
