@@ -412,7 +412,8 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
   if (PAIR) cluster_sync();  // both blocks' barriers exist before either is arrived on
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  grid_dependency_wait();
+  // The kernel before this one may still run. Every warp waits for it before it touches global memory, the
+  // producer and the scales warp after they have worked out where they will read.
   grid_dependency_trigger();
 
   if (warp == 0) {
@@ -424,6 +425,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
       for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
         int ta, tb;
         raster(t, p.tiles_a, p.tiles_b, ta, tb);
+        if (t == first_tile) grid_dependency_wait();
         for (int kb = kb_begin; kb < kb_end; ++kb) {
           if (!wait_or_abort(smem_u32(&empty_bar[stage]), phase ^ 1, abort_flag)) {
             if (!*abort_flag) record(p.status, 1, blockIdx.x, t, 100 + stage);
@@ -589,6 +591,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
       for (int c = 0; c < 4; ++c) row[c] = p.scales_a + min((PAIR ? ta * 2 + rank : ta) * kRowsA + c * 32 + lane, p.rows_a - 1) * p.scales_a_stride;
 #pragma unroll
       for (int c = 0; c < kRowsOfB; ++c) row[4 + c] = p.scales_b + min(tb * BN + c * 32 + lane, p.rows_b - 1) * p.scales_b_stride;
+      if (t == first_tile) grid_dependency_wait();
       for (int kb = kb_begin; kb < kb_end; kb += 4 * kSlotWords) {
         uint32_t w[4 + kRowsOfB][4];  // [32 rows each][word]
         load_scales<4 + kRowsOfB>(w, row, kb, p.k_blocks, align);
@@ -623,6 +626,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------------ epilogue
+    grid_dependency_wait();
     const int q = warp & 3;  // the lane quarter of tensor memory this warp may read
     uint8_t* my_staging = staging + q * kStagingSlots * kStagingBytes;
     int staged = 0, it = 0;
@@ -718,6 +722,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
   if (NARROW && p.split > 1) {
     // Every block of the cluster takes its share of the tile's (token, four columns) pieces and adds the
     // partial sums of all blocks in rank order.
+    grid_dependency_wait();  // at once by now: for the warps that have not waited yet
     cluster_sync();
     int ta, tb;
     raster(first_tile, p.tiles_a, p.tiles_b, ta, tb);
