@@ -69,7 +69,43 @@ struct Raw {
   uint32_t w[kWords];
 };
 
-// Loads the vector at `ptr`; elements from `valid` on are zero. VEC: vectors are 16-byte aligned and whole.
+// The vector at `ptr`, aligned to its elements only; elements from `valid` on are zero. The 16-byte pieces that
+// hold a valid element are loaded whole (such a piece is in the same page as that element) and the bytes
+// shifted into place, which costs two operations an element; loading them one by one took four times as long.
+template <typename T>
+__device__ __forceinline__ void load_shifted(Raw<T>& r, const T* ptr, int valid) {
+  constexpr int kPieces = Raw<T>::kWords / 4 + 1;
+  const uintptr_t address = reinterpret_cast<uintptr_t>(ptr);
+  const int offset = static_cast<int>(address & 15);
+  const uint4* piece = reinterpret_cast<const uint4*>(address & ~static_cast<uintptr_t>(15));
+  const int end = valid > 0 ? offset + valid * static_cast<int>(sizeof(T)) : 0;
+  uint32_t w[4 * kPieces];
+#pragma unroll
+  for (int i = 0; i < kPieces; ++i) {
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (16 * i < end) v = piece[i];
+    w[4 * i] = v.x;
+    w[4 * i + 1] = v.y;
+    w[4 * i + 2] = v.z;
+    w[4 * i + 3] = v.w;
+  }
+#pragma unroll
+  for (int i = 0; i + 2 < 4 * kPieces; ++i) w[i] = offset & 8 ? w[i + 2] : w[i];
+#pragma unroll
+  for (int i = 0; i + 3 < 4 * kPieces; ++i) w[i] = offset & 4 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < Raw<T>::kWords; ++i) r.w[i] = sizeof(T) == 2 ? __funnelshift_r(w[i], w[i + 1], (offset & 2) * 8) : w[i];
+  if (valid < kVec) {
+#pragma unroll
+    for (int i = 0; i < Raw<T>::kWords; ++i) {
+      constexpr int kPer = 4 / static_cast<int>(sizeof(T));  // elements of a word
+      const int left = valid - kPer * i;
+      r.w[i] &= left >= kPer ? 0xFFFFFFFFu : left == 1 && kPer == 2 ? 0xFFFFu : 0u;
+    }
+  }
+}
+
+// VEC: vectors are 16-byte aligned, and all or none of their elements valid.
 template <typename T, bool VEC>
 __device__ __forceinline__ void load_raw(Raw<T>& r, const T* ptr, int valid) {
   if constexpr (VEC) {
@@ -83,15 +119,7 @@ __device__ __forceinline__ void load_raw(Raw<T>& r, const T* ptr, int valid) {
       r.w[i + 3] = v.w;
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < Raw<T>::kWords; ++i) r.w[i] = 0;
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) {
-      if (i < valid) {
-        if constexpr (sizeof(T) == 4) r.w[i] = reinterpret_cast<const uint32_t*>(ptr)[i];
-        else r.w[i / 2] |= static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(ptr)[i]) << (16 * (i & 1));
-      }
-    }
+    load_shifted(r, ptr, valid);
   }
 }
 
@@ -138,13 +166,11 @@ __device__ __forceinline__ void store_as(T* ptr, const F2* v, int valid) {
   uint32_t w[Raw<T>::kWords];
 #pragma unroll
   for (int i = 0; i < kVec / 2; ++i) narrow(w, i, v[i], T());
-  if constexpr (VEC) {
-    if (valid > 0) {
+  if (VEC ? valid > 0 : valid >= kVec && (reinterpret_cast<uintptr_t>(ptr) & 15) == 0) {
 #pragma unroll
-      for (int i = 0; i < Raw<T>::kWords; i += 4)
-        *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(ptr) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-    }
-  } else {
+    for (int i = 0; i < Raw<T>::kWords; i += 4)
+      *reinterpret_cast<uint4*>(reinterpret_cast<uint32_t*>(ptr) + i) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
+  } else if (!VEC) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i) {
       if (i < valid) {
@@ -233,9 +259,9 @@ __device__ __forceinline__ uint32_t to_codes(F2 a, F2 b) {
 template <bool VEC>
 __device__ __forceinline__ void store_codes(uint8_t* ptr, const F2* v, F2 inverse, int valid) {
   const uint32_t lo = to_codes(mul2(v[0], inverse), mul2(v[1], inverse)), hi = to_codes(mul2(v[2], inverse), mul2(v[3], inverse));
-  if constexpr (VEC) {
-    if (valid > 0) *reinterpret_cast<uint2*>(ptr) = make_uint2(lo, hi);
-  } else {
+  if (VEC ? valid > 0 : valid >= kVec && (reinterpret_cast<uintptr_t>(ptr) & 7) == 0) {
+    *reinterpret_cast<uint2*>(ptr) = make_uint2(lo, hi);
+  } else if (!VEC) {
 #pragma unroll
     for (int i = 0; i < kVec; ++i)
       if (i < valid) ptr[i] = static_cast<uint8_t>((i < 4 ? lo : hi) >> (8 * (i & 3)));

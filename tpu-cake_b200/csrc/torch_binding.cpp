@@ -172,7 +172,7 @@ PyObject* rms_norm_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   Held held;
   if (a[7] != Py_None) {
     if (!rows_of(a[7], cols, scalar_type(dtype), "residual", device, x.count, &r)) return nullptr;
-    if (!(held.o[2] = output(a[10], x.count, cols, cols, scalar_type(dtype), "residual_out", device, &ro))) return nullptr;
+    if (!(held.o[2] = output(a[10], x.count, cols, (cols + 7) / 8 * 8, scalar_type(dtype), "residual_out", device, &ro))) return nullptr;
   } else {
     Py_INCREF(Py_None);
     held.o[2] = Py_None;
