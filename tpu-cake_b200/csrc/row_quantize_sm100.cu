@@ -418,11 +418,11 @@ struct NormParams {
   double inverse_cols;
 };
 
-// 1 / sqrt(a) as the sum of two f32: the f32 value by one Newton-Raphson step in double. A value next to the border
+// 1 / sqrt(a) as the sum of two f32: the hardware's estimate and one Newton-Raphson step in double. A value next to the border
 // of two codes goes to the wrong one by any error of the scale, and the whole row has the scale's; one step
 // in double costs six operations a thread. Zero and infinity pass through (their step is not a number).
 __device__ __forceinline__ void inverse_root(double a, float& hi, float& lo) {
-  const float y = 1.f / sqrtf(static_cast<float>(a));
+  const float y = rsqrtf(static_cast<float>(a));
   hi = y;
   lo = 0.f;
   if (y > 0.f && y < __int_as_float(0x7F800000)) {
@@ -442,13 +442,25 @@ __device__ __forceinline__ F2 scaled(F2 h, F2 hi, F2 minus_hi, F2 lo, F2 w) {
 
 // THREADS threads hold one row in registers, UNITS units of 16 elements each (unit i * THREADS + t of the row:
 // eight units are a group), so the sum x + residual is normalised as it is in 32 bits while its rounding is
-// stored, and the stored sum may lie over x or over the residual. Blocks have at least 256 threads, for
-// narrow rows several rows.
+// stored, and the stored sum may lie over x or over the residual. Without a residual there is little to load
+// for a row's chain of load, reduction, weights and store, so what counts then is that chain's length and how
+// many rows an SM has under way: THREADS follows the row closely, few registers, weights loaded
+// before the reduction where there is room for them, and the reduction itself short (f32 shuffles in a warp, two
+// to five steps between warps): 8192 x 5120 bf16 45 -> 29 us, 8192 x 2048 24 -> 15 us.
+__host__ __device__ constexpr int norm_rows(int threads) { return threads <= 128 ? 256 / threads : 1; }  // rows of a block
+
+__host__ __device__ constexpr int first_step(int v) {  // the first step of a reduction over v lanes
+  int d = 1;
+  while (2 * d < v) d *= 2;
+  return d;
+}
+
 template <typename T, typename W, int THREADS, int UNITS, bool VEC>
-__global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_quantize_sm100(const __grid_constant__ NormParams p) {
-  constexpr int kRows = THREADS < 256 ? 256 / THREADS : 1;  // rows of a block
-  constexpr int kWarps = THREADS / 32;                      // warps of a row
-  __shared__ double partial[kRows][kWarps];
+__global__ void __launch_bounds__(THREADS* norm_rows(THREADS)) cake_rms_norm_quantize_sm100(const __grid_constant__ NormParams p) {
+  constexpr int kRows = norm_rows(THREADS);
+  constexpr int kWarps = THREADS / 32;  // warps of a row
+  constexpr bool kEarlyWeights = UNITS == 1;
+  __shared__ float partial[kRows][kWarps];
   grid_dependency_wait();
   grid_dependency_trigger();
   const int t = threadIdx.x % THREADS;
@@ -458,6 +470,7 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
   // Column of unit i's first vector; the second is 64 further on.
   auto col_of = [&](int i) { return ((i * THREADS + t) / kGroupLanes) * kGroup + (t % kGroupLanes) * kVec; };
   F2 h[UNITS][kLaneVecs][kVec / 2];
+  Raw<W> early[kEarlyWeights ? kLaneVecs : 1];
   {
     Raw<T> x[UNITS][kLaneVecs], add[UNITS][kLaneVecs];
     const T* src = static_cast<const T*>(p.x) + static_cast<uint64_t>(row) * p.x_stride;
@@ -471,6 +484,13 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
         load_norm<T, VEC>(x[i][k], src + col, valid);
         if (p.residual) load_norm<T, VEC>(add[i][k], src_add + col, valid);
       }
+    if (kEarlyWeights) {
+#pragma unroll
+      for (int k = 0; k < kLaneVecs; ++k) {
+        const int col = col_of(0) + k * kGroupLanes * kVec;
+        load_norm<W, VEC>(early[kEarlyWeights ? k : 0], static_cast<const W*>(p.weight) + col, valid_at<VEC>(col, p.cols));
+      }
+    }
     T* dst = static_cast<T*>(p.residual_out) + static_cast<uint64_t>(row) * p.residual_out_stride;
 #pragma unroll
     for (int i = 0; i < UNITS; ++i)
@@ -494,16 +514,19 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
       for (int e = 0; e < kVec / 2; ++e) squares = fma2(h[i][k][e], h[i][k][e], squares);
   float even, odd;
   unpack2(squares, even, odd);
-  // 16 UNITS squares a thread in f32; between threads in double, where a rounding would be the whole row's.
-  double sum = static_cast<double>(even) + odd;
+  // 16 UNITS squares a thread and a warp's threads in f32; between warps in double, where a rounding would be
+  // the whole row's.
+  float in_warp = even + odd;
 #pragma unroll
-  for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+  for (int d = 16; d > 0; d >>= 1) in_warp += __shfl_xor_sync(0xffffffffu, in_warp, d);
+  double sum = in_warp;
   if (kWarps > 1) {
-    if ((t & 31) == 0) partial[r][t / 32] = sum;
+    if ((t & 31) == 0) partial[r][t / 32] = in_warp;
     __syncthreads();
-    sum = (t & 31) < kWarps ? partial[r][t & 31] : 0.0;
+    sum = (t & 31) < kWarps ? partial[r][t & 31] : 0.f;
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    for (int d = first_step(kWarps); d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    sum = __shfl_sync(0xffffffffu, sum, 0);
   }
   float hi, lo;
   inverse_root(sum * p.inverse_cols + static_cast<double>(p.epsilon), hi, lo);
@@ -515,7 +538,8 @@ __global__ void __launch_bounds__(THREADS < 256 ? 256 : THREADS) cake_rms_norm_q
     for (int k = 0; k < kLaneVecs; ++k) {
       const int col = col_of(i) + k * kGroupLanes * kVec;
       Raw<W> weight;  // from L1 or L2: every row of the SM reads them
-      load_norm<W, VEC>(weight, static_cast<const W*>(p.weight) + col, valid_at<VEC>(col, p.cols));
+      if (kEarlyWeights) weight = early[kEarlyWeights ? k : 0];
+      else load_norm<W, VEC>(weight, static_cast<const W*>(p.weight) + col, valid_at<VEC>(col, p.cols));
 #pragma unroll
       for (int e = 0; e < kVec / 2; ++e) {
         h[i][k][e] = scaled(h[i][k][e], hi2, minus_hi2, lo2, widen<W>(weight, e));
@@ -581,15 +605,24 @@ int32_t launch_quantize(const QuantizeParams& p, bool gate, bool vec, void* stre
   return launch(kernel, p, grid, kQuantThreads, stream);
 }
 
+template <typename T, typename W, int THREADS, int UNITS, bool VEC>
+int32_t launch_norm_as(const NormParams& p, void* stream) {
+  constexpr unsigned kRows = norm_rows(THREADS);
+  return launch(cake_rms_norm_quantize_sm100<T, W, THREADS, UNITS, VEC>, p, (p.rows + kRows - 1) / kRows, THREADS * kRows, stream);
+}
+
 template <typename T, typename W, bool VEC>
 int32_t launch_norm_vec(const NormParams& p, void* stream) {
   const int units = (p.cols + kGroup - 1) / kGroup * kGroupLanes;
-  if (units <= 32) return launch(cake_rms_norm_quantize_sm100<T, W, 32, 1, VEC>, p, (p.rows + 7) / 8, 256, stream);
-  if (units <= 64) return launch(cake_rms_norm_quantize_sm100<T, W, 32, 2, VEC>, p, (p.rows + 7) / 8, 256, stream);
-  if (units <= 256) return launch(cake_rms_norm_quantize_sm100<T, W, 128, 2, VEC>, p, (p.rows + 1) / 2, 256, stream);
-  if (units <= 512) return launch(cake_rms_norm_quantize_sm100<T, W, 256, 2, VEC>, p, p.rows, 256, stream);
-  if (units <= 1024) return launch(cake_rms_norm_quantize_sm100<T, W, 512, 2, VEC>, p, p.rows, 512, stream);
-  return launch(cake_rms_norm_quantize_sm100<T, W, 1024, 2, VEC>, p, p.rows, 1024, stream);
+  if (units <= 32) return launch_norm_as<T, W, 32, 1, VEC>(p, stream);
+  if (units <= 64) return launch_norm_as<T, W, 64, 1, VEC>(p, stream);
+  if (units <= 128) return launch_norm_as<T, W, 128, 1, VEC>(p, stream);
+  if (units <= 256) return launch_norm_as<T, W, 256, 1, VEC>(p, stream);
+  if (units <= 320) return launch_norm_as<T, W, 160, 2, VEC>(p, stream);
+  if (units <= 512) return launch_norm_as<T, W, 256, 2, VEC>(p, stream);
+  if (units <= 768) return launch_norm_as<T, W, 384, 2, VEC>(p, stream);
+  if (units <= 1024) return launch_norm_as<T, W, 512, 2, VEC>(p, stream);
+  return launch_norm_as<T, W, 1024, 2, VEC>(p, stream);
 }
 
 template <typename T>
