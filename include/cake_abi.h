@@ -321,8 +321,8 @@ int32_t cake_rms_norm_quantize_enqueue(const void* x, int32_t dtype, int64_t x_r
 /* out[m, n] = sum over k of lhs[m, k] * s_lhs[m, k / 128] * rhs[n, k] * s_rhs[n, k / 128], accumulated in
  * f32 and rounded once to out_dtype. */
 typedef struct cake_scaled_matmul_desc {
-  int64_t n;         /* rows of rhs = columns of out */
-  int64_t k;         /* contraction */
+  int64_t n;         /* rows of rhs = columns of out: 1 to 2^30 - 1 */
+  int64_t k;         /* contraction: 1 to 2^27 - 1 */
   int32_t out_dtype; /* CAKE_DTYPE_F32 or CAKE_DTYPE_BF16 */
   int32_t tile;      /* 0 = library default; 192, 224, 256: columns of a 256-row output tile;
                         16, 32, 64, 128: tokens of a tile of 128 rhs rows (few rows m) */

@@ -539,3 +539,23 @@ def test_invoke_refuses_wrong_operands(cuda_device):
             matmul.invoke(product, *wrong)
     with pytest.raises(ValueError, match="out must"):
         matmul.invoke(product, lhs, lhs_scales, rhs, rhs_scales, out=torch.zeros(4, 32, device=cuda_device))
+
+
+@pytest.mark.parametrize("tile, k_split", [(0, 0), (16, 1), (256, 0)])
+def test_matmul_longest_contraction(cuda_device, tile, k_split):
+    """2^27 - 1 codes a row, zero but for the first and the last of them: sums of 600 exact products."""
+    k = (1 << 27) - 1
+    sides = []
+    for seed, rows in ((1, 1), (2, 2)):
+        generator = torch.Generator().manual_seed(seed)
+        codes = torch.zeros(rows, -(-k // 16) * 16, dtype=torch.uint8, device=cuda_device).view(torch.float8_e4m3fn)[:, :k]
+        scales = torch.full((rows, -(-k // 128)), 126, dtype=torch.uint8, device=cuda_device).view(torch.float8_e8m0fnu)
+        values = torch.randint(-3, 4, (rows, 600), generator=generator).float()
+        codes[:, :300], codes[:, -300:] = values[:, :300].to(cuda_device).to(torch.float8_e4m3fn), values[:, 300:].to(cuda_device).to(torch.float8_e4m3fn)
+        sides.append((codes, scales, values))
+    expected = sides[0][2] @ sides[1][2].t() * 0.25
+    plan = scaled.CudaScaledMatmulPlan(name="t", n=2, k=k, output_dtype="f32", tile=tile, k_split=k_split)
+    executable = plan.build(cuda_device)
+    out = plan.invoke(executable, *sides[0][:2], *sides[1][:2])
+    assert executable.status() == (0, 0, 0, 0)
+    assert torch.equal(out.cpu(), expected)

@@ -48,7 +48,7 @@ def test_plans_refuse_what_they_do_not_run():
                       {"columns": 8, "epsilon": float("nan")}):
         with pytest.raises(ValueError):
             scaled.CudaRmsNormQuantizePlan(name="p", **arguments)
-    for arguments in ({"n": 0, "k": 8}, {"n": 8, "k": 0}, {"n": 1 << 30, "k": 8}, {"n": 8, "k": 8, "output_dtype": "f16"},
+    for arguments in ({"n": 0, "k": 8}, {"n": 8, "k": 0}, {"n": 1 << 30, "k": 8}, {"n": 8, "k": 1 << 27}, {"n": 8, "k": 8, "output_dtype": "f16"},
                       {"n": 8, "k": 8, "tile": 160}, {"n": 8, "k": 8, "tile": 256, "k_split": 2}, {"n": 8, "k": 8, "k_split": 2}, {"n": 8, "k": 8, "tile": 192, "k_split": 2},
                       {"n": 8, "k": 8, "tile": 16, "k_split": 9}):
         with pytest.raises(ValueError):
@@ -219,7 +219,8 @@ def _matmul(**overrides):
 
 @pytest.mark.parametrize("overrides, code, fragment", [
     ({"n": 0}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
-    ({"k": 1 << 31}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
+    ({"k": 1 << 27}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
+    ({"n": 1 << 30}, _native.CAKE_ERR_INVALID_ARGUMENT, "extents"),
     ({"out_dtype": 2}, _native.CAKE_ERR_INVALID_ARGUMENT, "out_dtype"),
     ({"tile": 160}, _native.CAKE_ERR_UNSUPPORTED, "tile"),
     ({"k_split": 9, "tile": 16}, _native.CAKE_ERR_INVALID_ARGUMENT, "k_split"),

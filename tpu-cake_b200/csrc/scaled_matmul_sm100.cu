@@ -49,7 +49,7 @@ constexpr int kUmmaK = 32;
 constexpr int kScaleSlots = 2;          // shared-memory ring of scales, 16 k blocks (four words a row) each
 constexpr int kSlotWords = 4;
 constexpr int kScaleSets = 3;           // sets of scale columns in tensor memory, used in turn
-constexpr int kStagingSlots = 2;        // 32 x 32 output chunks an epilogue warp may have in flight
+constexpr int kStagingSlots = 2;        // pieces of 32 rows x 128 bytes an epilogue warp may have in flight
 constexpr uint32_t kStagingBytes = 32 * 128;
 constexpr int kReducePitch = kRowsA + 4;  // floats between two tokens' partial sums
 constexpr long long kBudgetCycles = 4000000000ll;  // about two seconds of SM clock
@@ -88,7 +88,7 @@ struct Cfg {
 struct Params {
   int32_t rows_a, rows_b;    // rows of the two operands (wide: m and n; narrow: n and m)
   int32_t tiles_a, tiles_b;
-  int32_t k, k_blocks;
+  int32_t k_blocks;
   int32_t split;             // blocks of a cluster that share a tile (narrow)
   int32_t out_f32, tma_store;
   const uint8_t* scales_a;
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
   if (PAIR) cluster_sync();  // both blocks' barriers exist before either is arrived on
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
-  // The kernel before this one may still run. Every warp waits for it before it touches global memory, the
+  // The kernel before this one may still run. Every working warp waits for it before it does anything else, the
   // producer and the scales warp after they have worked out where they will read.
   grid_dependency_trigger();
 
@@ -465,6 +465,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
     // two k blocks shows as soon as it takes longer than one MMA. So this loop is kept to one wait, four
     // MMAs and one commit per k block (one more of each per four), with the control flow warp-uniform and
     // the descriptors stepped, not built.
+    grid_dependency_wait();  // its waits are bounded from here on
     const bool issuer = elect_one();
     const uint64_t desc0 = umma_desc_sw128(smem_u32(smem), 16, 1024);
     constexpr uint32_t kStageStep = C::kStageBytes >> 4;
@@ -541,6 +542,7 @@ __global__ void __launch_bounds__(kThreads, NARROW ? 2 : 1)
     if (lane == 0) {
       uint32_t slot = 0, slot_phase = 0, set = 0, set_phase = 0;
       bool ok = true;
+      grid_dependency_wait();
       for (int t = first_tile; t < num_tiles && ok; t += tile_step) {
         for (int kb = kb_begin; kb < kb_end; kb += 4) {
           const int word = ((kb - kb_begin) / 4) % kSlotWords;
@@ -883,9 +885,10 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
                                    void* out, int64_t out_row_stride, int32_t* status_device, void* stream) {
   if (!desc) return fail(CAKE_ERR_INVALID_ARGUMENT, "cake_scaled_matmul_enqueue: null argument");
   const cake_scaled_matmul_desc& d = *desc;
-  // Rows and columns are tensor-map coordinates; a tile past the end must not wrap around either.
-  if (d.n < 1 || d.k < 1 || d.n > INT32_MAX / 2 || d.k > INT32_MAX / 2)
-    return fail(CAKE_ERR_INVALID_ARGUMENT, "scaled matmul extents must be 1 to 2^30 - 1: n=%lld k=%lld", (long long)d.n, (long long)d.k);
+  // Rows and columns are tensor-map coordinates; a tile past the end must not wrap around either. A tile's
+  // contraction has to end well within the two seconds that a wait may take: 2^20 k blocks take 0.4.
+  if (d.n < 1 || d.n > INT32_MAX / 2 || d.k < 1 || d.k >= (1 << 27))
+    return fail(CAKE_ERR_INVALID_ARGUMENT, "scaled matmul extents must be n = 1 to 2^30 - 1 and k = 1 to 2^27 - 1: n=%lld k=%lld", (long long)d.n, (long long)d.k);
   if (d.out_dtype != CAKE_DTYPE_F32 && d.out_dtype != CAKE_DTYPE_BF16)
     return fail(CAKE_ERR_INVALID_ARGUMENT, "out_dtype must be CAKE_DTYPE_F32 or CAKE_DTYPE_BF16");
   if (d.tile != 0 && d.tile != 16 && d.tile != 32 && d.tile != 64 && d.tile != 128 && d.tile != 192 && d.tile != 224 && d.tile != 256)
@@ -936,7 +939,6 @@ int32_t cake_scaled_matmul_enqueue(const cake_scaled_matmul_desc* desc, int64_t 
     return fail(CAKE_ERR_UNSUPPORTED, "%lld x %lld tiles are more than one launch covers", (long long)tiles_a, (long long)tiles_b);
   p.tiles_a = static_cast<int32_t>(tiles_a);
   p.tiles_b = static_cast<int32_t>(tiles_b);
-  p.k = static_cast<int32_t>(d.k);
   p.k_blocks = static_cast<int32_t>(k_blocks);
   p.split = c.split;
   p.out_f32 = osize == 4;

@@ -189,8 +189,8 @@ class CudaScaledMatmulPlan:
     k_split: int = 0
 
     def __post_init__(self) -> None:
-        if not (0 < self.n < 1 << 30 and 0 < self.k < 1 << 30):
-            raise ValueError(f"scaled matmul extents must be 1 to 2^30 - 1, got n={self.n} k={self.k}")
+        if not (0 < self.n < 1 << 30 and 0 < self.k < 1 << 27):
+            raise ValueError(f"scaled matmul extents must be n = 1 to 2^30 - 1 and k = 1 to 2^27 - 1, got n={self.n} k={self.k}")
         if self.output_dtype not in ("bf16", "f32"):
             raise ValueError(f"output dtype must be f32 or bf16, got {self.output_dtype}")
         if self.tile not in (0, 16, 32, 64, 128, 192, 224, 256):
